@@ -25,6 +25,9 @@ OBJ = os.path.join(os.path.dirname(PKG), "build", "obj")
 OUT = os.path.join(PKG, "_C.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
+# no packed fp32 instructions: some of their forms have given wrong results on
+# MI355X now and then (the host pass warns that it does not know the feature)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _torch_paths():
@@ -52,7 +55,7 @@ def _run(cmd):
 def build(verbose: bool = False, force: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     inc, tlib, cxx11 = _torch_paths()
-    headers = glob.glob(os.path.join(CSRC, "*.h"))
+    headers = glob.glob(os.path.join(CSRC, "*.h")) + [os.path.abspath(__file__)]  # (its flags)
     hip_srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     cpp_srcs = sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
     hipcc = os.path.join(ROCM, "bin", "hipcc")
@@ -63,7 +66,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
         o = os.path.join(OBJ, os.path.basename(s) + ".o")
         if force or _newer(s, o, headers):
             jobs.append([hipcc, "-c", "-fPIC", "-O3", "-std=c++17", f"--offload-arch={ARCH}",
-                         "-munsafe-fp-atomics", "-Wall", "-I", CSRC, s, "-o", o])
+                         "-munsafe-fp-atomics", *NO_PACKED_FP32, "-Wall", "-I", CSRC, s, "-o", o])
     abi = f"-D_GLIBCXX_USE_CXX11_ABI={int(cxx11)}"
     for s in cpp_srcs:
         o = os.path.join(OBJ, os.path.basename(s) + ".o")
