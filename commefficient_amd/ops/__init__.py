@@ -1,6 +1,7 @@
 """Native codec ops (HIP gfx950 + C++ CPU): Count Sketch, deterministic top-k,
 fused server/client state updates, DP clip+noise, download accounting and
-on-device augmentation.  See ``csrc/`` for the kernels."""
+on-device augmentation, and generation from a paged key-value cache
+(``decode``).  See ``csrc/`` for the kernels."""
 from __future__ import annotations
 
 from typing import Optional, Tuple
@@ -8,6 +9,8 @@ from typing import Optional, Tuple
 import torch
 
 from .._ext import ops as _ops
+from .decode import (PagedKV, beam_reorder, beam_select, kv_extend, kv_write,
+                     paged_attention)
 from .sketch import CSVec, make_hashes
 
 __all__ = ["CSVec", "make_hashes", "topk_abs", "topk_dense", "momentum_ef", "sparse_apply",
@@ -179,3 +182,4 @@ def client_means(out, rows, slot, counts) -> None:
 
 
 __all__ += ["conv_weight_prep", "conv3x3_fwd", "conv3x3_wgrad", "relu_mask", "client_means"]
+__all__ += ["PagedKV", "beam_reorder", "beam_select", "kv_extend", "kv_write", "paged_attention"]
