@@ -66,8 +66,10 @@ struct PagedAttnArgs {
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;         // elements
   int64_t kc_page, kc_head, kc_tok, vc_page, vc_head, vc_tok;  // elements
   int64_t table_ld, pages;
-  int n, heads, kv_heads, dim, width, page, split;
+  int n, heads, kv_heads, dim, width, page;
   float scale;
+  int split, waves;  // plan_paged_attention
+  uint32_t magic;
 };
 
 struct BeamSelectArgs {
@@ -87,7 +89,8 @@ void launch_kv_extend(const KvExtendArgs& a, hipStream_t stream);
 void launch_kv_write(const KvWriteArgs& a, hipStream_t stream);
 void launch_beam_reorder(const BeamReorderArgs& a, hipStream_t stream);
 void launch_paged_attention(const PagedAttnArgs& a, DecodeType t, hipStream_t stream);
-int paged_attention_split(int n, int kv_heads, int group, int64_t longest);
+// fills split, waves and magic; longest: a hint of the longest sequence
+void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest);
 void launch_beam_select(const BeamSelectArgs& a, DecodeType t, hipStream_t stream);
 int beam_select_parts(int vocab);
 

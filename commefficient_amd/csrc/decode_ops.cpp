@@ -353,6 +353,9 @@ void check_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
   same_device(table, kc, op, "table");
   check_i32(lens, q.size(0), kc, op, "lens");
   check_page(kc.size(2), table.size(1), op);
+  TORCH_CHECK(kc.size(0) >= 1 && kc.size(0) * kc.size(2) < (1ll << 31), op,
+              ": the caches must hold 1 to 2^31 - 1 slots, not ", kc.size(0), " pages of ", kc.size(2));
+  TORCH_CHECK(q.size(0) * q.size(1) <= (1ll << 24), op, ": at most 2^24 sequences x heads");
   TORCH_CHECK(given(k) == given(v), op, ": k and v come together");
   if (given(k)) {
     check_rows(*k, q.size(0), kc, op, "k");
@@ -402,14 +405,15 @@ at::Tensor paged_attention_hip(const at::Tensor& q_, at::Tensor kc, at::Tensor v
   a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(a.dim)));
   const int64_t most = std::min<int64_t>(longest.has_value() ? std::max<int64_t>(1, *longest) : (1ll << 30),
                                          static_cast<int64_t>(a.width) * a.page);
-  a.split = paged_attention_split(a.n, a.kv_heads, a.heads / a.kv_heads, most);
+  const DecodeType type = decode_type(kc, "paged_attention", "the key cache");
+  plan_paged_attention(a, type, most);
   a.part = nullptr;
   at::Tensor part;
   if (a.split > 1) {
     part = at::empty({static_cast<int64_t>(a.n) * a.heads * a.split * (a.dim + 2)}, q.options().dtype(at::kFloat));
     a.part = part.data_ptr<float>();
   }
-  launch_paged_attention(a, decode_type(kc, "paged_attention", "the key cache"), stream_now());
+  launch_paged_attention(a, type, stream_now());
   return out;
 }
 

@@ -3,138 +3,436 @@
 // t < lens[n], the keys read through table[n].  When the new token's own k, v
 // rows are given they stand for position lens[n] - 1 and are stored into that
 // slot by the same launch.  Rows without tokens, or with every score -inf, are
-// 0; a row that meets a page
-// id outside the cache, or is longer than its table row, is NaN and nothing
-// is read or written through that id.
+// 0; a row that meets a page id outside the cache, or is longer than its table
+// row, is NaN and nothing is read or written through that id.
+//
+// Every key and value is read once for all `group` query heads that share it
+// and used for 4 x group operations a number: bound by HBM, so the kernel is
+// built around its loads.  A wave takes 32 tokens at a time of one (sequence,
+// cache head); the group's heads (up to 16, the rest of the columns idle: the
+// MFMA time is under a tenth of the loads' even so) are the columns of both
+// products, computed transposed:
+//   S^T [token, head] = K Q^T,   O^T [column, head] += V^T P^T.
+// The MFMA's row order is free as long as both sides agree, and is chosen so
+// that nothing moves between lanes:
+//   * row m of key set s (s = 0, 1) is token 8 (m / 4) + 4 s + m % 4, so that
+//     lane l's eight scores are tokens 8 (l / 16) .. + 7 of head l % 16: the
+//     very operand layout that the second product wants for P^T;
+//   * a lane loads 8 tokens x head_dim / 16 columns of V and transposes them
+//     within its own registers (v_perm_b32) into rows of V^T.
+// So K and V go from memory to the matrix cores without LDS.  Weights are fed
+// as two 16-bit pieces (a rounding and its remainder: 2^-16 of a weight for
+// bf16, 2^-22 for fp16), sums and maxima stay in fp32; fp32 caches use the
+// fp32 MFMA.  The running maximum is only raised when some score exceeds it
+// by kSlack (in powers of two), which a wave votes on: the cross-lane maximum
+// and the rescaling of O run a few times a sequence, not once a tile.
 #include <hip/hip_runtime.h>
-#include <hip/hip_fp16.h>
+#include <cfloat>
 #include <cstdint>
+#include "conv_common.h"
 #include "decode.h"
 
 namespace commeff {
 namespace {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kTile = 32;  // tokens a wave takes at a time
 
 template <DecodeType T>
 struct Elem;
 template <>
 struct Elem<kBf16> {
   typedef uint16_t t;
-  static __device__ __forceinline__ float load(t x) { return __uint_as_float(static_cast<uint32_t>(x) << 16); }
-  static __device__ __forceinline__ t store(float f) {
-    return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));
+  static constexpr float kSlack = 8.f, kLift = 0.f;
+  static __device__ __forceinline__ t store(float f) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f)); }
+  static __device__ __forceinline__ float load(t x) { return bf2f(x); }
+  static __device__ __forceinline__ f32x4_t mfma(v4u a, v4u b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                   c, 0, 0, 0);
   }
 };
 template <>
 struct Elem<kF16> {
   typedef uint16_t t;
-  static __device__ __forceinline__ float load(t x) { return static_cast<float>(__builtin_bit_cast(_Float16, x)); }
+  // weights reach 2^(1 + 12) < 65,504 and the smallest kept piece is 2^-24 / 2^12
+  static constexpr float kSlack = 1.f, kLift = 12.f;
   static __device__ __forceinline__ t store(float f) {
     return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
+  }
+  static __device__ __forceinline__ float load(t x) { return static_cast<float>(__builtin_bit_cast(_Float16, x)); }
+  static __device__ __forceinline__ f32x4_t mfma(v4u a, v4u b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                  0, 0, 0);
   }
 };
 template <>
 struct Elem<kF32> {
   typedef float t;
-  static __device__ __forceinline__ float load(t x) { return x; }
+  static constexpr float kSlack = 8.f, kLift = 0.f;
   static __device__ __forceinline__ t store(float f) { return f; }
 };
 
-// a workgroup per (sequence, query head), a wave per token, a lane per column
-template <DecodeType T>
-__global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnArgs a) {
+// waves of a workgroup where there are few workgroups: as many as leave each
+// the registers of two tiles (1,024 / 512 threads: 128 / 256 a lane)
+constexpr int many_waves(int type, int dim) {
+  const int row = dim * (type == kF32 ? 4 : 2);
+  return row <= 128 ? 16 : row <= 256 ? 8 : 4;
+}
+
+// waves a SIMD holds at least of a 4-wave workgroup's kernel
+constexpr int min_waves(int type, int dim) {
+  const int row = dim * (type == kF32 ? 4 : 2);
+  return row <= 64 ? 4 : row <= 128 ? 3 : row <= 256 ? 2 : 1;
+}
+
+// what a lane holds of 32 tokens: dwords of K rows and of V columns
+template <DecodeType T, int HD>
+struct Tile {
+  static constexpr int E = T == kF32 ? 4 : 2;      // bytes an element
+  static constexpr int KL = HD * E / 64;           // 16-byte pieces a K row leaves to a lane
+  static constexpr int NC = HD / 16;               // V columns a lane holds
+  static constexpr int CH = NC * E > 16 ? 16 / E : NC;  // .. of them in one load
+  v4u k[2][KL];
+  uint32_t v[8][NC * E / 4];
+};
+// column j of lane row m (of 16)
+template <DecodeType T, int HD>
+__device__ __forceinline__ int v_col(int m, int j) {
+  constexpr int CH = Tile<T, HD>::CH;
+  return (j / CH) * (16 * CH) + m * CH + j % CH;
+}
+
+template <DecodeType T, int HD, int W>
+__global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) paged_attn_kernel(PagedAttnArgs a) {
   typedef Elem<T> E;
   typedef typename E::t S;
-  const int n = blockIdx.x / a.heads, h = blockIdx.x - n * a.heads;
-  const int kh = h / (a.heads / a.kv_heads);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  typedef Tile<T, HD> Regs;
+  constexpr int NC = Regs::NC, KL = Regs::KL, CH = Regs::CH, EB = Regs::E;
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // W x min(group, 16) x (HD + 2)
+
+  const int group = a.heads / a.kv_heads, tiles16 = (group + 15) >> 4;
+  // neighbours in the batch (the beams of a request, which share pages) on one XCD
+  int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int n = id % a.n;
+  id /= a.n;
+  const int kh = id % a.kv_heads;
+  id /= a.kv_heads;
+  const int gt = id % tiles16, sp = id / tiles16;
+  const int cols = min(16, group - 16 * gt);  // query heads of this workgroup
+  const int h0 = kh * group + 16 * gt;
+
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m16 = lane & 15, g = lane >> 4;
   const int len = a.lens[n];
-  S* out = static_cast<S*>(a.out) + (static_cast<int64_t>(n) * a.heads + h) * a.dim;
-  if (len <= 0) {
-    for (int d = tid; d < a.dim; d += 256) out[d] = E::store(0.f);
-    return;
-  }
   bool bad = len > static_cast<int64_t>(a.width) * a.page;
-  const int32_t* row = a.table + n * a.table_ld;
-  const S* q = static_cast<const S*>(a.q) + n * a.q_row + h * a.q_head;
+  const int all = len > 0 && !bad ? (len + kTile - 1) / kTile : 0;  // tiles of the sequence
+  const int per = (all + a.split - 1) / a.split;
+  const int t_end = min(all, (sp + 1) * per);
+  if (sp > 0 && sp * per >= all) return;  // (the join knows)
+
   const S* kn = a.k ? static_cast<const S*>(a.k) + n * a.k_row + kh * a.k_head : nullptr;
-  const S* vn = a.v ? static_cast<const S*>(a.v) + n * a.v_row + kh * a.v_head : nullptr;
-  S* kc = static_cast<S*>(a.kc) + kh * a.kc_head;
-  S* vc = static_cast<S*>(a.vc) + kh * a.vc_head;
-  constexpr int MD = 4;  // 64-column pieces of a head of at most 256
-  float qv[MD], acc[MD];
+  const S* vn = a.k ? static_cast<const S*>(a.v) + n * a.v_row + kh * a.v_head : nullptr;
+  S* const kc = static_cast<S*>(a.kc) + kh * a.kc_head;
+  S* const vc = static_cast<S*>(a.vc) + kh * a.vc_head;
+  const int32_t* row = a.table + n * a.table_ld;
+
+  auto page_of = [&](int tok) {  // tok / page, exact for tok < 2^30: see launch_paged_attention
+    int q = static_cast<int>(__umulhi(static_cast<uint32_t>(tok), a.magic));
+    q -= q * a.page > tok;
+    return a.page == 1 ? tok : q;
+  };
+  const bool by8 = (a.page & 7) == 0;  // eight aligned tokens lie in one page
+  auto look = [&](int tile) {  // the page of token lane % 32 of a tile; one outside the cache is not followed
+    const int tok = tile * kTile + (lane & 31);
+    const int pid = tok < len ? row[page_of(tok)] : 0;
+    const bool ok = pid >= 0 && pid < a.pages;
+    bad |= !ok;
+    return ok ? pid : 0;
+  };
+  auto load = [&](int tile, int ids, Regs& r) {
+    const int base = tile * kTile;
+    const bool edge = base + kTile > len - 1;  // the last token is not read from the cache, those behind it not at all
+    int pid = __shfl(ids, 8 * (m16 >> 2), 64);
 #pragma unroll
-  for (int i = 0; i < MD; ++i) {
-    const int d = lane + 64 * i;
-    qv[i] = d < a.dim ? E::load(q[d]) * a.scale : 0.f;
-    acc[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  if (!bad) {
-    for (int t = w; t < len; t += 4) {
-      const int64_t id = row[t / a.page];
-      if (id < 0 || id >= a.pages) {
-        bad = true;  // (the new token is stored all the same, through its own page)
-        continue;
+    for (int s = 0; s < 2; ++s) {
+      const int at = 8 * (m16 >> 2) + 4 * s + (m16 & 3), tok = base + at;
+      if (!by8) pid = __shfl(ids, at, 64);
+      const S* kr = kc + pid * a.kc_page + (tok - page_of(tok) * a.page) * a.kc_tok;
+      if (edge && kn && tok == len - 1) kr = kn;
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        r.k[s][i] = v4u{0u, 0u, 0u, 0u};
+        if (!edge || tok < len) r.k[s][i] = *reinterpret_cast<const v4u*>(kr + i * (64 / EB) + g * (16 / EB));
       }
-      const int64_t off = t % a.page;
-      const bool fresh = kn && t == len - 1;
-      S* kslot = kc + id * a.kc_page + off * a.kc_tok;
-      S* vslot = vc + id * a.vc_page + off * a.vc_tok;
-      const S* kr = fresh ? kn : kslot;
-      const S* vr = fresh ? vn : vslot;
-      float x = 0.f, v[MD];
+    }
+    const int first = base + 8 * g;
+    pid = __shfl(ids, 8 * g, 64);
+    const S* vr = vc + pid * a.vc_page + (first - page_of(first) * a.page) * a.vc_tok;
 #pragma unroll
-      for (int i = 0; i < MD; ++i) {
-        const int d = lane + 64 * i;
-        v[i] = 0.f;
-        if (d < a.dim) {
-          x += qv[i] * E::load(kr[d]);
-          v[i] = E::load(vr[d]);
-          if (fresh && h % (a.heads / a.kv_heads) == 0) {
-            kslot[d] = kr[d];
-            vslot[d] = vr[d];
-          }
+    for (int i = 0; i < 8; ++i) {
+      const int tok = first + i;
+      const S* x = vr + i * a.vc_tok;
+      if (!by8) x = vc + __shfl(ids, 8 * g + i, 64) * a.vc_page + (tok - page_of(tok) * a.page) * a.vc_tok;
+      if (edge && kn && tok == len - 1) x = vn;
+#pragma unroll
+      for (int c = 0; c < NC / CH; ++c) {
+        const S* src = x + v_col<T, HD>(m16, c * CH);
+        uint32_t* dst = &r.v[i][c * CH * EB / 4];
+        if constexpr (CH * EB == 16) {
+          v4u u = {0u, 0u, 0u, 0u};
+          if (!edge || tok < len) u = *reinterpret_cast<const v4u*>(src);
+          dst[0] = u[0], dst[1] = u[1], dst[2] = u[2], dst[3] = u[3];
+        } else if constexpr (CH * EB == 8) {
+          v2u u = {0u, 0u};
+          if (!edge || tok < len) u = *reinterpret_cast<const v2u*>(src);
+          dst[0] = u[0], dst[1] = u[1];
+        } else {
+          dst[0] = 0u;
+          if (!edge || tok < len) dst[0] = *reinterpret_cast<const uint32_t*>(src);
         }
       }
-      for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-      const float mn = fmaxf(m, x), at = mn == -INFINITY ? 0.f : mn;  // (all scores -inf: weights 0)
-      const float c = __expf(m - at), p = __expf(x - at);
-      m = mn;
-      l = l * c + p;
+    }
+  };
+
+  // Q^T: lane l holds head l % 16, the columns that it holds of a K row
+  v4u q[KL];
 #pragma unroll
-      for (int i = 0; i < MD; ++i) acc[i] = acc[i] * c + p * v[i];
+  for (int i = 0; i < KL; ++i) {
+    q[i] = v4u{0u, 0u, 0u, 0u};
+    if (m16 < cols)
+      q[i] = *reinterpret_cast<const v4u*>(static_cast<const S*>(a.q) + n * a.q_row + (h0 + m16) * a.q_head +
+                                           i * (64 / EB) + g * (16 / EB));
+  }
+  const float scale = a.scale * 1.44269504088896340736f;  // scores in powers of two
+  float top = -FLT_MAX, sum = 0.f;                        // of head l % 16; sum: this lane's tokens
+  f32x4_t o[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](int tile, const Regs& r) {
+    f32x4_t s4[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      s4[s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        if constexpr (T == kF32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s4[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(r.k[s][i][e]), __uint_as_float(q[i][e]),
+                                                         s4[s], 0, 0, 0);
+        } else {
+          s4[s] = E::mfma(r.k[s][i], q[i], s4[s]);
+        }
+      }
+    }
+    float x[8], most = -INFINITY;
+    const int first = tile * kTile + 8 * g;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = s4[i >> 2][i & 3] * scale;
+      if (first + i >= len) x[i] = -INFINITY;
+      most = fmaxf(most, x[i]);
+    }
+    if (__any(m16 < cols && most > top + E::kSlack)) {
+      most = fmaxf(most, __shfl_xor(most, 16, 64));
+      most = fmaxf(most, __shfl_xor(most, 32, 64));
+      const float now = fmaxf(top, most), c = exp2f(top - now);
+      top = now;
+      sum *= c;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) o[j] *= c;
+    }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = exp2f(x[i] - top + E::kLift);
+      sum += p[i];
+    }
+    if constexpr (T == kF32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(r.v[i][j]), p[i], o[j], 0, 0, 0);
+    } else {
+      v4u hi, lo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u0 = E::store(p[2 * i]), u1 = E::store(p[2 * i + 1]);
+        hi[i] = u0 | u1 << 16;
+        lo[i] = E::store(p[2 * i] - E::load(u0)) | static_cast<uint32_t>(E::store(p[2 * i + 1] - E::load(u1))) << 16;
+      }
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        v4u vt;  // row j of V^T: the lane's eight tokens
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          vt[i] = __builtin_amdgcn_perm(r.v[2 * i + 1][j >> 1], r.v[2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+        o[j] = E::mfma(vt, hi, o[j]);
+        o[j] = E::mfma(vt, lo, o[j]);
+      }
+    }
+  };
+
+  const int t0 = sp * per + w;
+  if constexpr (HD * EB <= 512) {  // the next tile's loads run under this one's products
+    if (t0 < t_end) {
+      Regs cur, nxt;
+      load(t0, look(t0), cur);
+      int ids = t0 + W < t_end ? look(t0 + W) : 0;
+      for (int t = t0; t < t_end; t += W) {
+        if (t + W < t_end) load(t + W, ids, nxt);
+        if (t + 2 * W < t_end) ids = look(t + 2 * W);
+        compute(t, cur);
+        if (t + W < t_end) cur = nxt;
+      }
+    }
+  } else {
+    for (int t = t0; t < t_end; t += W) {
+      Regs cur;
+      load(t, look(t), cur);
+      compute(t, cur);
     }
   }
-  __shared__ float sm[4], sl[4], so[4][256];
-  if (lane == 0) {
-    sm[w] = m;
-    sl[w] = bad ? NAN : l;
+
+  // the new row into its slot, by the workgroup that holds the last token
+  if (kn && len > 0 && gt == 0 && len <= static_cast<int64_t>(a.width) * a.page && t_end == all && w == W - 1) {
+    const int pg = page_of(len - 1), pid = row[pg];
+    if (pid >= 0 && pid < a.pages) {
+      const int64_t off = len - 1 - pg * a.page;
+      for (int c = lane; c < HD * EB / 16; c += 64) {
+        reinterpret_cast<v4u*>(kc + pid * a.kc_page + off * a.kc_tok)[c] = reinterpret_cast<const v4u*>(kn)[c];
+        reinterpret_cast<v4u*>(vc + pid * a.vc_page + off * a.vc_tok)[c] = reinterpret_cast<const v4u*>(vn)[c];
+      }
+    }
   }
+
+  sum += __shfl_xor(sum, 16, 64);
+  sum += __shfl_xor(sum, 32, 64);
+  if (__any(bad)) sum = NAN;
+  float* lo = lds + static_cast<size_t>(w) * cols * HD;            // [W][cols][HD]
+  float* lms = lds + static_cast<size_t>(W) * cols * HD;           // [W][cols] maxima, then sums
+  if (m16 < cols) {
+    if (g == 0) {
+      lms[w * cols + m16] = top;
+      lms[(W + w) * cols + m16] = sum;
+    }
 #pragma unroll
-  for (int i = 0; i < MD; ++i) so[w][lane + 64 * i] = acc[i];
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) lo[m16 * HD + v_col<T, HD>(4 * g + r, j)] = o[j][r];
+  }
   __syncthreads();
-  const float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  for (int d = tid; d < a.dim; d += 256) {
+  for (int x = tid; x < cols * HD; x += W * 64) {
+    const int c = x / HD, d = x - c * HD;
+    float mm = lms[c];
+#pragma unroll
+    for (int i = 1; i < W; ++i) mm = fmaxf(mm, lms[i * cols + c]);
     float num = 0.f, den = 0.f;
-    for (int i = 0; i < 4; ++i) {
-      const float c = sm[i] == -INFINITY ? 0.f : __expf(sm[i] - mm);
-      num += c * so[i][d];
-      den += sl[i] != sl[i] ? NAN : c * sl[i];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float f = exp2f(lms[i * cols + c] - mm);
+      num += f * lds[i * cols * HD + x];
+      den += f * lms[(W + i) * cols + c];
     }
-    out[d] = E::store(den == 0.f ? 0.f : num / den);
+    const int64_t at = static_cast<int64_t>(n) * a.heads + h0 + c;
+    if (a.split == 1) {
+      static_cast<S*>(a.out)[at * HD + d] = E::store(den == 0.f ? 0.f : num / den);
+    } else {
+      float* part = a.part + (at * a.split + sp) * (HD + 2);
+      part[d] = num;
+      if (d == 0) part[HD] = mm, part[HD + 1] = den;
+    }
   }
+}
+
+// the parts of a split sequence, in their order
+template <DecodeType T>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnArgs a) {
+  typedef Elem<T> E;
+  const int64_t at = blockIdx.x;
+  const int n = static_cast<int>(at / a.heads);
+  const int len = a.lens[n];
+  const bool over = len > static_cast<int64_t>(a.width) * a.page;
+  const int all = len > 0 && !over ? (len + kTile - 1) / kTile : 0;
+  const int per = (all + a.split - 1) / a.split;
+  const int parts = per > 0 ? (all + per - 1) / per : 1;
+  const float* part = a.part + at * a.split * (a.dim + 2);
+  for (int d = threadIdx.x; d < a.dim; d += 256) {
+    float mm = -FLT_MAX;
+    for (int i = 0; i < parts; ++i) mm = fmaxf(mm, part[i * (a.dim + 2) + a.dim]);
+    float num = 0.f, den = 0.f;
+    for (int i = 0; i < parts; ++i) {
+      const float* p = part + i * (a.dim + 2);
+      const float f = exp2f(p[a.dim] - mm);
+      num += f * p[d];
+      den += f * p[a.dim + 1];
+    }
+    static_cast<typename E::t*>(a.out)[at * a.dim + d] = E::store(den == 0.f ? 0.f : num / den);
+  }
+}
+
+template <DecodeType T, int HD, int W>
+void launch_one(const PagedAttnArgs& a, hipStream_t stream) {
+  const int group = a.heads / a.kv_heads, cols = group < 16 ? group : 16;
+  const uint32_t lds = static_cast<uint32_t>(W * cols * (HD + 2) * 4);
+  if (lds > 65536) {
+    static bool attr = false;
+    if (!attr) {
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, HD, W>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+      attr = true;
+    }
+  }
+  const uint32_t blocks = static_cast<uint32_t>(a.n) * a.kv_heads * ((group + 15) / 16) * a.split;
+  COMMEFF_LAUNCH((paged_attn_kernel<T, HD, W>), dim3(blocks), dim3(W * 64), lds, stream, a);
+  if (a.split > 1)
+    COMMEFF_LAUNCH(paged_attn_join_kernel<T>, dim3(static_cast<uint32_t>(a.n) * a.heads), dim3(256), 0, stream, a);
+}
+
+template <DecodeType T, int HD>
+void launch_dim(const PagedAttnArgs& a, hipStream_t stream) {
+  constexpr int kMany = many_waves(T, HD);
+  if constexpr (kMany > 4) {
+    if (a.waves == kMany) return launch_one<T, HD, kMany>(a, stream);
+  }
+  launch_one<T, HD, 4>(a, stream);
+}
+
+template <DecodeType T>
+void launch_type(const PagedAttnArgs& a, hipStream_t stream) {
+  if (a.dim == 32) launch_dim<T, 32>(a, stream);
+  else if (a.dim == 64) launch_dim<T, 64>(a, stream);
+  else if (a.dim == 128) launch_dim<T, 128>(a, stream);
+  else launch_dim<T, 256>(a, stream);
 }
 
 }  // namespace
 
-int paged_attention_split(int, int, int, int64_t) { return 1; }
+// Waves a workgroup and parts a sequence: a workgroup serves one (sequence,
+// cache head, 16 query heads), its waves take the sequence's tiles in turn.
+void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest) {
+  const int group = a.heads / a.kv_heads, cols = group < 16 ? group : 16;
+  const int64_t groups = static_cast<int64_t>(a.n) * a.kv_heads * ((group + 15) / 16);
+  const int64_t tiles = (longest + kTile - 1) / kTile;
+  a.waves = groups < 512 && cols * a.dim <= 1024 ? many_waves(t, a.dim) : 4;
+  int64_t split = (512 + groups - 1) / (groups > 0 ? groups : 1);
+  const int64_t most = tiles / (2 * a.waves);
+  split = split > most ? most : split;
+  a.split = static_cast<int>(split < 1 ? 1 : split > 128 ? 128 : split);
+  // q = umulhi(x, 2^32 / page + 1) is x / page or one more for x < 2^30: it
+  // adds at most x (page / 2^32) / page < 1
+  a.magic = a.page == 1 ? 0u : static_cast<uint32_t>((1ull << 32) / static_cast<uint64_t>(a.page) + 1);
+}
 
 void launch_paged_attention(const PagedAttnArgs& a, DecodeType t, hipStream_t stream) {
   if (a.n == 0) return;
-  const dim3 grid(static_cast<uint32_t>(a.n) * a.heads);
-  if (t == kBf16) COMMEFF_LAUNCH(paged_attn_kernel<kBf16>, grid, dim3(256), 0, stream, a);
-  else if (t == kF16) COMMEFF_LAUNCH(paged_attn_kernel<kF16>, grid, dim3(256), 0, stream, a);
-  else COMMEFF_LAUNCH(paged_attn_kernel<kF32>, grid, dim3(256), 0, stream, a);
+  if (t == kBf16) launch_type<kBf16>(a, stream);
+  else if (t == kF16) launch_type<kF16>(a, stream);
+  else launch_type<kF32>(a, stream);
 }
 
 }  // namespace commeff
