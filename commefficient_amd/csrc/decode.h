@@ -78,8 +78,8 @@ struct BeamSelectArgs {
   const uint8_t* finished;  // [requests, beams] or null
   float* out_scores;        // [requests, keep]
   int64_t *out_parent, *out_token;
-  unsigned long long* cand;  // workspace
-  float* stat;
+  unsigned long long* cand;  // workspace [requests * beams, parts, keep]
+  double* stat;              // workspace [requests * beams, parts, 2]
   int64_t s_request, s_beam;  // elements
   int64_t eos;
   int requests, beams, vocab, keep, parts;
@@ -92,6 +92,6 @@ void launch_paged_attention(const PagedAttnArgs& a, DecodeType t, hipStream_t st
 // fills split, waves and magic; longest: a hint of the longest sequence
 void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest);
 void launch_beam_select(const BeamSelectArgs& a, DecodeType t, hipStream_t stream);
-int beam_select_parts(int vocab);
+int beam_select_parts(int vocab, DecodeType t);
 
 }  // namespace commeff

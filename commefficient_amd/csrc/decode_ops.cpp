@@ -487,6 +487,8 @@ void check_select(const at::Tensor& logits, const at::Tensor& scores, int64_t ke
   TORCH_CHECK(logits.dim() == 3 && logits.size(1) >= 1 && logits.size(2) >= 1, op,
               ": logits must be [requests, beams, vocabulary], not ", logits.sizes());
   TORCH_CHECK(logits.size(1) * logits.size(2) <= (1ll << 31) - 1, op, ": beams x vocabulary must be below 2^31");
+  TORCH_CHECK(logits.size(1) <= 1024 && logits.size(0) * logits.size(1) <= 65535, op,
+              ": at most 1,024 beams and 65,535 rows, not ", logits.size(0), " x ", logits.size(1));
   no_grad(logits, op, "logits");
   TORCH_CHECK(scores.scalar_type() == at::kFloat && scores.dim() == 2 && scores.is_contiguous() &&
                   scores.size(0) == logits.size(0) && scores.size(1) == logits.size(1),
@@ -530,10 +532,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_hip(const at::Tensor&
   a.beams = static_cast<int>(x.size(1));
   a.vocab = static_cast<int>(x.size(2));
   a.keep = static_cast<int>(keep);
-  a.parts = beam_select_parts(a.vocab);
-  a.cand = nullptr;
-  a.stat = nullptr;
-  launch_beam_select(a, decode_type(x, "beam_select", "logits"), stream_now());
+  const DecodeType type = decode_type(x, "beam_select", "logits");
+  a.parts = beam_select_parts(a.vocab, type);
+  const int64_t lists = scores.numel() * a.parts;
+  auto work = at::empty({lists * (keep + 2)}, scores.options().dtype(at::kLong));
+  a.cand = reinterpret_cast<unsigned long long*>(work.data_ptr<int64_t>());
+  a.stat = reinterpret_cast<double*>(a.cand + lists * keep);
+  launch_beam_select(a, type, stream_now());
   return out;
 }
 
