@@ -11,101 +11,172 @@ namespace {
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------ extend
-// inclusive scan over a 1,024-thread block (16 waves); `total` is its sum
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int64_t* total) {
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
-  __syncthreads();  // (lds is free again)
-  if (lane == 63) lds[w] = v;
-  __syncthreads();
-  int64_t before = 0, all = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if (i < w) before += lds[i];
-    all += lds[i];
-  }
-  *total = all;
-  return v + before;
-}
-
 // With e_i the tokens asked for (negative: none) and c(x) = ceil(x / page):
 //   start_i = sum_{j<i} e_j,  need_i = c(len_i + e_i) - c(len_i),
 // sequence i is served if its counts are sound, its table row and the output
 // rows are long enough and the pool holds the pages that it and all sequences
 // before it need; its pages are pool[used + sum_{j<i} need_j ..].  Row r of
 // sequence i is token p = len_i + r - start_i, slot table[i][p / page] * page
-// + p % page.  One workgroup: two scans over the sequences, then the rows.
-__global__ void __launch_bounds__(1024) kv_extend_kernel(KvExtendArgs a) {
-  __shared__ int64_t lds[16];
+// + p % page.  A few hundred KB at most: bound by latency, that is by the
+// launch, two scans and the chain row -> sequence -> page.  So one workgroup
+// does all of it with the sequences' plan in LDS; only batches too large for
+// that (kFused) leave the rows to a second launch over the whole chip.
+constexpr int kScan = 1024, kEach = 4;  // threads of the scan, sequences a thread takes at once
+constexpr int kFused = 8192;            // sequences and rows of a single launch
+
+// inclusive scan of min(a + b, cap) over the block, values <= cap <= 2^30 + 1;
+// `total`: all of it
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t cap, uint32_t* lds, uint32_t* total) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t u = __shfl_up(v, o, 64);
+    if (lane >= o) v = min(u + v, cap);
+  }
+  __syncthreads();  // (lds is free again)
+  if (lane == 63) lds[w] = v;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kScan / 64; ++i) {
+    if (i == w) before = all;
+    all = min(all + lds[i], cap);
+  }
+  *total = all;
+  return min(before + v, cap);
+}
+
+struct KvPlan {  // of the sequences: LDS, or global memory
+  int32_t *start, *base, *first;
+};
+
+// row r: its slot, position and sequence, and the table entry where it opens a page
+__device__ __forceinline__ void extend_row(const KvExtendArgs& a, const KvPlan& p, int r) {
+  int lo = 0, hi = a.n;  // the first sequence that ends past r
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (p.start[mid + 1] > r) hi = mid;
+    else lo = mid + 1;
+  }
+  int64_t slot = -1;
+  int pos = 0;
+  if (lo < a.n) {
+    const int len = p.base[lo];
+    if (len >= 0) {
+      pos = len + r - p.start[lo];
+      const int pi = static_cast<uint32_t>(pos) / static_cast<uint32_t>(a.page);
+      const int have = static_cast<uint32_t>(len + a.page - 1) / static_cast<uint32_t>(a.page);
+      int32_t* row = a.table + lo * a.table_ld;
+      int64_t id;
+      if (pi < have) {
+        id = row[pi];
+      } else {
+        id = a.pool[p.first[lo] + pi - have];
+        if (pos == pi * a.page) row[pi] = static_cast<int32_t>(id);
+      }
+      if (id >= 0) slot = id * a.page + (pos - pi * a.page);
+    }
+  }
+  a.slots[r] = slot;
+  a.pos[r] = pos;
+  a.seq[r] = lo < a.n ? lo : -1;
+}
+
+template <bool FUSED>
+__global__ void __launch_bounds__(kScan) kv_extend_kernel(KvExtendArgs a) {
+  extern __shared__ int32_t s_plan[];  // FUSED: start [n + 1] | base [n] | first [n]
+  __shared__ uint32_t lds[kScan / 64];
+  __shared__ int s_got, s_miss;
   const int tid = threadIdx.x;
-  const int64_t used = a.used[0];
-  const int64_t avail = used < 0 ? 0 : (a.pool_n > used ? a.pool_n - used : 0);
-  int64_t rows_before = 0, need_before = 0, got = 0, miss = 0;
-  for (int i0 = 0; i0 < a.n; i0 += 1024) {
-    const int i = i0 + tid;
-    const bool in = i < a.n;
-    const int64_t len = in ? a.lens[i] : 0, fresh = in ? a.fresh[i] : 0;
-    int64_t total;
-    const int64_t add = fresh > 0 ? fresh : 0;
-    const int64_t end = rows_before + block_scan(add, lds, &total);
-    rows_before += total;
-    const bool fits = in && fresh >= 0 && len >= 0 && end <= a.rows &&
-                      len + fresh <= static_cast<int64_t>(a.width) * a.page;
-    const int64_t need = fits ? (len + fresh + a.page - 1) / a.page - (len + a.page - 1) / a.page : 0;
-    const int64_t upto = need_before + block_scan(need, lds, &total);
-    need_before += total;
-    const bool served = fits && (need == 0 || upto <= avail);
-    if (in) {
-      a.start[i] = static_cast<int32_t>(end - add < a.rows ? end - add : a.rows);
-      if (i == a.n - 1) a.start[a.n] = static_cast<int32_t>(end < a.rows ? end : a.rows);
-      a.base[i] = served ? static_cast<int32_t>(len) : -1;
-      a.first[i] = static_cast<int32_t>(used + (served ? upto - need : 0));
-      a.lens_out[i] = static_cast<int32_t>(served ? len + fresh : len);
+  KvPlan p = {a.start, a.base, a.first};
+  if constexpr (FUSED) p = {s_plan, s_plan + a.n + 1, s_plan + 2 * a.n + 1};
+  if (tid == 0) s_got = s_miss = 0;
+  const int used = a.used[0];
+  const uint32_t avail = used < 0 || used > a.pool_n ? 0u : static_cast<uint32_t>(a.pool_n - used);
+  const uint32_t rows = static_cast<uint32_t>(a.rows), page = static_cast<uint32_t>(a.page);
+  uint32_t rows_before = 0, need_before = 0;  // saturated at rows + 1 and avail + 1
+  int got = 0, miss = 0;
+  for (int i0 = 0; i0 < a.n; i0 += kScan * kEach) {
+    const int i = i0 + tid * kEach;
+    int len[kEach], fresh[kEach];
+    uint32_t end[kEach], upto[kEach], need[kEach], total;
+    bool fits[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      len[k] = i + k < a.n ? a.lens[i + k] : 0;
+      fresh[k] = i + k < a.n ? a.fresh[i + k] : 0;
     }
-    block_scan(served ? need : 0, lds, &total);
-    got += total;
-    block_scan(in && !served ? 1 : 0, lds, &total);
-    miss += total;
-  }
-  if (a.n == 0 && tid == 0) a.start[0] = 0;
-  __syncthreads();  // start, base and first of every sequence are written; used was read
-  if (tid == 0) {
-    a.used_out[0] = static_cast<int32_t>(used + got);
-    a.missed[0] = static_cast<int32_t>(miss);
-  }
-  for (int r = tid; r < a.rows; r += 1024) {
-    int lo = 0, hi = a.n;  // the first sequence that ends past r
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (a.start[mid + 1] > r) hi = mid;
-      else lo = mid + 1;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+      end[k] = min((k ? end[k - 1] : 0u) + min(static_cast<uint32_t>(max(fresh[k], 0)), rows + 1), rows + 1);
+    const uint32_t rb = rows_before;
+    uint32_t mine = end[kEach - 1];
+    uint32_t incl = block_scan(mine, rows + 1, lds, &total);
+    // (what lies before this thread: the scan without its own, which saturation forbids to subtract)
+    uint32_t prev = __shfl_up(incl, 1, 64);
+    if ((tid & 63) == 0) {
+      prev = 0;
+      for (int w = 0; w < (tid >> 6); ++w) prev = min(prev + lds[w], rows + 1);
     }
-    int64_t slot = -1;
-    int pos = 0;
-    if (lo < a.n) {
-      const int len = a.base[lo];
-      if (len >= 0) {
-        pos = len + r - a.start[lo];
-        const int pi = pos / a.page, have = (len + a.page - 1) / a.page;
-        int32_t* row = a.table + static_cast<int64_t>(lo) * a.table_ld;
-        int64_t id;
-        if (pi < have) {
-          id = row[pi];
-        } else {
-          id = a.pool[a.first[lo] + pi - have];
-          if (pos == pi * a.page) row[pi] = static_cast<int32_t>(id);
-        }
-        if (id >= 0) slot = id * a.page + (pos - pi * a.page);
+    prev = min(rb + prev, rows + 1);
+    rows_before = min(rb + total, rows + 1);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const uint32_t begin = k ? min(prev + end[k - 1], rows + 1) : prev, e = min(prev + end[k], rows + 1);
+      fits[k] = i + k < a.n && fresh[k] >= 0 && len[k] >= 0 && e <= rows &&
+                static_cast<int64_t>(len[k]) + fresh[k] <= static_cast<int64_t>(a.width) * a.page;
+      need[k] = 0;
+      if (fits[k])
+        need[k] = (static_cast<uint32_t>(len[k] + fresh[k]) + page - 1) / page -
+                  (static_cast<uint32_t>(len[k]) + page - 1) / page;
+      upto[k] = min((k ? upto[k - 1] : 0u) + min(need[k], avail + 1), avail + 1);
+      if (i + k < a.n) {
+        p.start[i + k] = static_cast<int32_t>(min(begin, rows));
+        if constexpr (FUSED) a.start[i + k] = static_cast<int32_t>(min(begin, rows));
       }
     }
-    a.slots[r] = slot;
-    a.pos[r] = pos;
-    a.seq[r] = lo < a.n ? lo : -1;
+    const uint32_t nb = need_before;
+    mine = upto[kEach - 1];
+    incl = block_scan(mine, avail + 1, lds, &total);
+    prev = __shfl_up(incl, 1, 64);
+    if ((tid & 63) == 0) {
+      prev = 0;
+      for (int w = 0; w < (tid >> 6); ++w) prev = min(prev + lds[w], avail + 1);
+    }
+    prev = min(nb + prev, avail + 1);
+    need_before = min(nb + total, avail + 1);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (i + k >= a.n) break;
+      const uint32_t u = min(prev + upto[k], avail + 1);
+      const bool served = fits[k] && (need[k] == 0 || u <= avail);
+      p.base[i + k] = served ? len[k] : -1;
+      p.first[i + k] = served ? used + static_cast<int>(u - need[k]) : 0;
+      a.lens_out[i + k] = served ? len[k] + fresh[k] : len[k];
+      if (served && need[k]) got = static_cast<int>(u);  // (the last one served has them all before it)
+      miss += !served;
+    }
   }
+  __syncthreads();  // s_got and s_miss are set, `used` was read
+  if (got) atomicMax(&s_got, got);
+  if (miss) atomicAdd(&s_miss, miss);
+  if (tid == 0) {
+    const int32_t last = static_cast<int32_t>(min(rows_before, rows));
+    p.start[a.n] = last;
+    if constexpr (FUSED) a.start[a.n] = last;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    a.used_out[0] = used + s_got;
+    a.missed[0] = s_miss;
+  }
+  if constexpr (FUSED)
+    for (int r = tid; r < a.rows; r += kScan) extend_row(a, p, r);
+}
+
+__global__ void __launch_bounds__(256) kv_extend_rows_kernel(KvExtendArgs a) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r < a.rows) extend_row(a, KvPlan{a.start, a.base, a.first}, r);
 }
 
 // ------------------------------------------------------------------- write
@@ -209,7 +280,22 @@ void reorder_unit(const BeamReorderArgs& a, hipStream_t stream) {
 }  // namespace
 
 void launch_kv_extend(const KvExtendArgs& a, hipStream_t stream) {
-  COMMEFF_LAUNCH(kv_extend_kernel, dim3(1), dim3(1024), 0, stream, a);
+  if (a.n <= kFused && a.rows <= kFused) {
+    const uint32_t lds = static_cast<uint32_t>(3 * a.n + 1) * 4;
+    if (lds > 48 * 1024) {
+      static bool attr = false;
+      if (!attr) {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kv_extend_kernel<true>),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (3 * kFused + 1) * 4);
+        attr = true;
+      }
+    }
+    COMMEFF_LAUNCH(kv_extend_kernel<true>, dim3(1), dim3(kScan), lds, stream, a);
+    return;
+  }
+  COMMEFF_LAUNCH(kv_extend_kernel<false>, dim3(1), dim3(kScan), 0, stream, a);
+  if (a.rows > 0)
+    COMMEFF_LAUNCH(kv_extend_rows_kernel, dim3(static_cast<uint32_t>((a.rows + 255) / 256)), dim3(256), 0, stream, a);
 }
 
 void launch_kv_write(const KvWriteArgs& a, hipStream_t stream) {

@@ -80,6 +80,13 @@ def _extend_case(name):
         n = 1027
         lens = torch.randint(0, 60, (n,), generator=g).tolist()
         return torch.randint(0, 5000, (n, 4), generator=g), lens, [1] * n, 600, 0, 16, n
+    if name == "crowd":  # more sequences than one launch plans, the pool's end among them
+        n = 9001
+        lens = torch.randint(0, 60, (n,), generator=g).tolist()
+        return torch.randint(0, 5000, (n, 4), generator=g), lens, torch.randint(-1, 3, (n,), generator=g).tolist(), \
+            900, 3, 16, 3 * n
+    if name == "row":  # one sequence takes them all
+        return torch.full((5000, 3), 4), [0] * 5000, [0] * 4444 + [33] + [0] * 555, 50, 0, 16, 40
     if name == "long":
         return torch.full((3, 3000), -1), [0, 0, 0], [2900, 17, 2999], 9000, 0, 1, 6000
     raise KeyError(name)
@@ -91,7 +98,7 @@ def hash_of(name):
 
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("name", ["none", "prompt", "mixed", "refused", "exhausted", "spent", "many", "step",
-                                  "long"])
+                                  "long", "crowd", "row"])
 @pytest.mark.parametrize("device", DEVICES)
 def test_extend(device, name, in_place):
     table, lens, new, pages, used, page, rows = _extend_case(name)
