@@ -6,13 +6,33 @@
 // int32 names each sequence's pages in order, lens [sequences] int32 counts
 // its tokens.  A page id outside [0, pages) is never followed.
 #pragma once
+#ifdef __HIPCC__
+#include <hip/hip_runtime.h>
+#else
 #include <hip/hip_runtime_api.h>
+#endif
 #include <cstdint>
 #include "launch.h"
 
 namespace commeff {
 
 enum DecodeType { kBf16 = 0, kF16 = 1, kF32 = 2 };
+
+// x / d for 0 <= x < 2^31 by a product: umulhi(x, 2^32 / d + 1) is the quotient
+// or one more (it adds at most x / 2^32 to x / d)
+struct FastDiv {
+  uint32_t d, m;
+#ifdef __HIPCC__
+  __device__ __forceinline__ int of(int x) const {
+    uint32_t q = __umulhi(static_cast<uint32_t>(x), m);
+    q -= q * d > static_cast<uint32_t>(x);
+    return d == 1 ? x : static_cast<int>(q);
+  }
+#endif
+};
+inline FastDiv fast_div(int64_t d) {
+  return {static_cast<uint32_t>(d < 1 ? 1 : d), d <= 1 ? 0u : static_cast<uint32_t>((1ull << 32) / d + 1)};
+}
 
 constexpr int kBeamMaxKeep = 64;     // candidates of one beam_select request
 constexpr int kReorderMaxBeams = 32;
@@ -68,8 +88,8 @@ struct PagedAttnArgs {
   int64_t table_ld, pages;
   int n, heads, kv_heads, dim, width, page;
   float scale;
-  int split, waves;  // plan_paged_attention
-  uint32_t magic;
+  int split, waves, group;  // plan_paged_attention
+  FastDiv by_heads, by_n, by_kv, by_tiles, by_split, by_page;
 };
 
 struct BeamSelectArgs {
@@ -89,7 +109,7 @@ void launch_kv_extend(const KvExtendArgs& a, hipStream_t stream);
 void launch_kv_write(const KvWriteArgs& a, hipStream_t stream);
 void launch_beam_reorder(const BeamReorderArgs& a, hipStream_t stream);
 void launch_paged_attention(const PagedAttnArgs& a, DecodeType t, hipStream_t stream);
-// fills split, waves and magic; longest: a hint of the longest sequence
+// fills in the split and the divisors; longest: a hint of the longest sequence
 void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest);
 void launch_beam_select(const BeamSelectArgs& a, DecodeType t, hipStream_t stream);
 int beam_select_parts(int vocab, DecodeType t);

@@ -39,7 +39,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
-constexpr int kTile = 32;  // tokens a wave takes at a time
+constexpr int kTile = 32;       // tokens a wave takes at a time
+constexpr int kMaxSplit = 128;  // parts of a sequence
 
 template <DecodeType T>
 struct Elem;
@@ -113,22 +114,30 @@ __global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) page
   constexpr int NC = Regs::NC, KL = Regs::KL, CH = Regs::CH, EB = Regs::E;
   extern __shared__ __attribute__((aligned(16))) float lds[];  // W x min(group, 16) x (HD + 2)
 
-  const int group = a.heads / a.kv_heads, tiles16 = (group + 15) >> 4;
   // neighbours in the batch (the beams of a request, which share pages) on one XCD
   int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int n = id % a.n;
-  id /= a.n;
-  const int kh = id % a.kv_heads;
-  id /= a.kv_heads;
-  const int gt = id % tiles16, sp = id / tiles16;
-  const int cols = min(16, group - 16 * gt);  // query heads of this workgroup
-  const int h0 = kh * group + 16 * gt;
+  int q0 = a.by_n.of(id);
+  const int n = id - q0 * a.n;
+  id = q0;
+  q0 = a.by_kv.of(id);
+  const int kh = id - q0 * a.kv_heads;
+  id = q0;
+  const int sp = a.by_tiles.of(id), gt = id - sp * static_cast<int>(a.by_tiles.d);
+  const int cols = min(16, a.group - 16 * gt);  // query heads of this workgroup
+  const int h0 = kh * a.group + 16 * gt;
 
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m16 = lane & 15, g = lane >> 4;
+  const int32_t* row = a.table + n * a.table_ld;
   const int len = a.lens[n];
+  // the first tile's page ids do not wait for the length where its place does not depend on it
+  int early = 0;
+  if (a.split == 1) {
+    const int pg = a.by_page.of(w * kTile + (lane & 31));
+    early = pg < a.width ? row[pg] : 0;
+  }
   bool bad = len > static_cast<int64_t>(a.width) * a.page;
   const int all = len > 0 && !bad ? (len + kTile - 1) / kTile : 0;  // tiles of the sequence
-  const int per = (all + a.split - 1) / a.split;
+  const int per = a.split == 1 ? all : a.by_split.of(all + a.split - 1);
   const int t_end = min(all, (sp + 1) * per);
   if (sp > 0 && sp * per >= all) return;  // (the join knows)
 
@@ -136,61 +145,67 @@ __global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) page
   const S* vn = a.k ? static_cast<const S*>(a.v) + n * a.v_row + kh * a.v_head : nullptr;
   S* const kc = static_cast<S*>(a.kc) + kh * a.kc_head;
   S* const vc = static_cast<S*>(a.vc) + kh * a.vc_head;
-  const int32_t* row = a.table + n * a.table_ld;
 
-  auto page_of = [&](int tok) {  // tok / page, exact for tok < 2^30: see launch_paged_attention
-    int q = static_cast<int>(__umulhi(static_cast<uint32_t>(tok), a.magic));
-    q -= q * a.page > tok;
-    return a.page == 1 ? tok : q;
-  };
+  // Tokens behind the last one read the last one's page instead: their scores
+  // are masked and their V pieces cleared before the product.
+  const int last = len - 1;
   const bool by8 = (a.page & 7) == 0;  // eight aligned tokens lie in one page
-  auto look = [&](int tile) {  // the page of token lane % 32 of a tile; one outside the cache is not followed
-    const int tok = tile * kTile + (lane & 31);
-    const int pid = tok < len ? row[page_of(tok)] : 0;
+  auto sound = [&](int pid) {  // a page outside the cache is not followed
     const bool ok = pid >= 0 && pid < a.pages;
     bad |= !ok;
     return ok ? pid : 0;
   };
+  auto look = [&](int tile) {  // the page of token lane % 32 of a tile
+    return sound(row[a.by_page.of(min(tile * kTile + (lane & 31), last))]);
+  };
   auto load = [&](int tile, int ids, Regs& r) {
     const int base = tile * kTile;
-    const bool edge = base + kTile > len - 1;  // the last token is not read from the cache, those behind it not at all
-    int pid = __shfl(ids, 8 * (m16 >> 2), 64);
+    const bool fresh = kn && base + kTile > last;  // the tile with the new token
+    const S *kr[2], *vr[8];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int at = 8 * (m16 >> 2) + 4 * s + (m16 & 3), tok = base + at;
-      if (!by8) pid = __shfl(ids, at, 64);
-      const S* kr = kc + pid * a.kc_page + (tok - page_of(tok) * a.page) * a.kc_tok;
-      if (edge && kn && tok == len - 1) kr = kn;
+      const int at = min(8 * (m16 >> 2) + 4 * s + (m16 & 3), last - base), tok = base + at;
+      kr[s] = kc + __shfl(ids, at, 64) * a.kc_page + (tok - a.by_page.of(tok) * a.page) * a.kc_tok;
+    }
+    if (by8) {
+      const int at = min(8 * g, (last - base) & ~7), tok = base + at;
+      vr[0] = vc + __shfl(ids, at, 64) * a.vc_page + (tok - a.by_page.of(tok) * a.page) * a.vc_tok;
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        r.k[s][i] = v4u{0u, 0u, 0u, 0u};
-        if (!edge || tok < len) r.k[s][i] = *reinterpret_cast<const v4u*>(kr + i * (64 / EB) + g * (16 / EB));
+      for (int i = 1; i < 8; ++i) vr[i] = vr[i - 1] + a.vc_tok;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = min(8 * g + i, last - base), tok = base + at;
+        vr[i] = vc + __shfl(ids, at, 64) * a.vc_page + (tok - a.by_page.of(tok) * a.page) * a.vc_tok;
       }
     }
-    const int first = base + 8 * g;
-    pid = __shfl(ids, 8 * g, 64);
-    const S* vr = vc + pid * a.vc_page + (first - page_of(first) * a.page) * a.vc_tok;
+    if (fresh) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (base + 8 * (m16 >> 2) + 4 * s + (m16 & 3) == last) kr[s] = kn;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (base + 8 * g + i == last) vr[i] = vn;
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < KL; ++i)
+        r.k[s][i] = *reinterpret_cast<const v4u*>(kr[s] + i * (64 / EB) + g * (16 / EB));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int tok = first + i;
-      const S* x = vr + i * a.vc_tok;
-      if (!by8) x = vc + __shfl(ids, 8 * g + i, 64) * a.vc_page + (tok - page_of(tok) * a.page) * a.vc_tok;
-      if (edge && kn && tok == len - 1) x = vn;
 #pragma unroll
       for (int c = 0; c < NC / CH; ++c) {
-        const S* src = x + v_col<T, HD>(m16, c * CH);
+        const S* src = vr[i] + v_col<T, HD>(m16, c * CH);
         uint32_t* dst = &r.v[i][c * CH * EB / 4];
         if constexpr (CH * EB == 16) {
-          v4u u = {0u, 0u, 0u, 0u};
-          if (!edge || tok < len) u = *reinterpret_cast<const v4u*>(src);
+          const v4u u = *reinterpret_cast<const v4u*>(src);
           dst[0] = u[0], dst[1] = u[1], dst[2] = u[2], dst[3] = u[3];
         } else if constexpr (CH * EB == 8) {
-          v2u u = {0u, 0u};
-          if (!edge || tok < len) u = *reinterpret_cast<const v2u*>(src);
+          const v2u u = *reinterpret_cast<const v2u*>(src);
           dst[0] = u[0], dst[1] = u[1];
         } else {
-          dst[0] = 0u;
-          if (!edge || tok < len) dst[0] = *reinterpret_cast<const uint32_t*>(src);
+          dst[0] = *reinterpret_cast<const uint32_t*>(src);
         }
       }
     }
@@ -211,7 +226,16 @@ __global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) page
 #pragma unroll
   for (int j = 0; j < NC; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  auto compute = [&](int tile, const Regs& r) {
+  auto compute = [&](int tile, Regs& r) {
+    const int first = tile * kTile + 8 * g;
+    if (tile * kTile + kTile > len) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (first + i >= len) {
+#pragma unroll
+          for (int c = 0; c < NC * EB / 4; ++c) r.v[i][c] = 0u;
+        }
+    }
     f32x4_t s4[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -229,7 +253,6 @@ __global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) page
       }
     }
     float x[8], most = -INFINITY;
-    const int first = tile * kTile + 8 * g;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       x[i] = s4[i >> 2][i & 3] * scale;
@@ -278,31 +301,33 @@ __global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) page
   };
 
   const int t0 = sp * per + w;
-  if constexpr (HD * EB <= 512) {  // the next tile's loads run under this one's products
-    if (t0 < t_end) {
+  if (t0 < t_end) {
+    int ids = a.split == 1 ? sound(t0 * kTile + (lane & 31) <= last ? early : 0) : look(t0);
+    if constexpr (HD * EB <= 512) {  // the next tile's loads run under this one's products
       Regs cur, nxt;
-      load(t0, look(t0), cur);
-      int ids = t0 + W < t_end ? look(t0 + W) : 0;
-      for (int t = t0; t < t_end; t += W) {
-        if (t + W < t_end) load(t + W, ids, nxt);
-        if (t + 2 * W < t_end) ids = look(t + 2 * W);
-        compute(t, cur);
-        if (t + W < t_end) cur = nxt;
+      for (int t = t0; t < t_end + W; t += W) {  // (one copy of each: the code, too, has to be read)
+        if (t < t_end) {
+          load(t, ids, nxt);
+          if (t + W < t_end) ids = look(t + W);
+        }
+        if (t > t0) compute(t - W, cur);
+        cur = nxt;
       }
-    }
-  } else {
-    for (int t = t0; t < t_end; t += W) {
-      Regs cur;
-      load(t, look(t), cur);
-      compute(t, cur);
+    } else {
+      for (int t = t0; t < t_end; t += W) {
+        Regs cur;
+        load(t, ids, cur);
+        if (t + W < t_end) ids = look(t + W);
+        compute(t, cur);
+      }
     }
   }
 
   // the new row into its slot, by the workgroup that holds the last token
   if (kn && len > 0 && gt == 0 && len <= static_cast<int64_t>(a.width) * a.page && t_end == all && w == W - 1) {
-    const int pg = page_of(len - 1), pid = row[pg];
+    const int pg = a.by_page.of(last), pid = row[pg];
     if (pid >= 0 && pid < a.pages) {
-      const int64_t off = len - 1 - pg * a.page;
+      const int64_t off = last - pg * a.page;
       for (int c = lane; c < HD * EB / 16; c += 64) {
         reinterpret_cast<v4u*>(kc + pid * a.kc_page + off * a.kc_tok)[c] = reinterpret_cast<const v4u*>(kn)[c];
         reinterpret_cast<v4u*>(vc + pid * a.vc_page + off * a.vc_tok)[c] = reinterpret_cast<const v4u*>(vn)[c];
@@ -349,29 +374,45 @@ __global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) page
   }
 }
 
-// the parts of a split sequence, in their order
+// the parts of a split sequence: 256 threads, 256 / dim of them to a column
 template <DecodeType T>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnArgs a) {
   typedef Elem<T> E;
-  const int64_t at = blockIdx.x;
-  const int n = static_cast<int>(at / a.heads);
+  __shared__ float s_w[kMaxSplit], s_num[256], s_top[4], s_den[4];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int at = blockIdx.x, n = a.by_heads.of(at);
   const int len = a.lens[n];
   const bool over = len > static_cast<int64_t>(a.width) * a.page;
   const int all = len > 0 && !over ? (len + kTile - 1) / kTile : 0;
-  const int per = (all + a.split - 1) / a.split;
-  const int parts = per > 0 ? (all + per - 1) / per : 1;
-  const float* part = a.part + at * a.split * (a.dim + 2);
-  for (int d = threadIdx.x; d < a.dim; d += 256) {
-    float mm = -FLT_MAX;
-    for (int i = 0; i < parts; ++i) mm = fmaxf(mm, part[i * (a.dim + 2) + a.dim]);
-    float num = 0.f, den = 0.f;
-    for (int i = 0; i < parts; ++i) {
-      const float* p = part + i * (a.dim + 2);
-      const float f = exp2f(p[a.dim] - mm);
-      num += f * p[d];
-      den += f * p[a.dim + 1];
-    }
-    static_cast<typename E::t*>(a.out)[at * a.dim + d] = E::store(den == 0.f ? 0.f : num / den);
+  const int per = a.by_split.of(all + a.split - 1);
+  int parts = 1;  // those that some workgroup wrote
+  if (per > 0) parts = (all + per - 1) / per;
+  const float* part = a.part + static_cast<int64_t>(at) * a.split * (a.dim + 2);
+  float top = -FLT_MAX, den = 0.f;
+  if (tid < parts) top = part[tid * (a.dim + 2) + a.dim], den = part[tid * (a.dim + 2) + a.dim + 1];
+  float m = top;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if (lane == 0) s_top[w] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  const float f = exp2f(top - m);
+  if (tid < kMaxSplit) s_w[tid] = f;
+  den *= f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
+  if (lane == 0) s_den[w] = den;
+  __syncthreads();
+  const int d = tid & (a.dim - 1), step = 256 / a.dim;
+  float num = 0.f;
+#pragma unroll 8
+  for (int i = tid / a.dim; i < parts; i += step) num += s_w[i] * part[i * (a.dim + 2) + d];
+  s_num[tid] = num;
+  __syncthreads();
+  if (tid < a.dim) {
+    for (int i = 1; i < step; ++i) num += s_num[tid + i * a.dim];
+    den = s_den[0] + s_den[1] + s_den[2] + s_den[3];
+    static_cast<typename E::t*>(a.out)[static_cast<int64_t>(at) * a.dim + d] = E::store(den == 0.f ? 0.f : num / den);
   }
 }
 
@@ -422,10 +463,14 @@ void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest) {
   int64_t split = (512 + groups - 1) / (groups > 0 ? groups : 1);
   const int64_t most = tiles / (2 * a.waves);
   split = split > most ? most : split;
-  a.split = static_cast<int>(split < 1 ? 1 : split > 128 ? 128 : split);
-  // q = umulhi(x, 2^32 / page + 1) is x / page or one more for x < 2^30: it
-  // adds at most x (page / 2^32) / page < 1
-  a.magic = a.page == 1 ? 0u : static_cast<uint32_t>((1ull << 32) / static_cast<uint64_t>(a.page) + 1);
+  a.split = static_cast<int>(split < 1 ? 1 : split > kMaxSplit ? kMaxSplit : split);
+  a.group = group;
+  a.by_heads = fast_div(a.heads);
+  a.by_n = fast_div(a.n);
+  a.by_kv = fast_div(a.kv_heads);
+  a.by_tiles = fast_div((group + 15) / 16);
+  a.by_split = fast_div(a.split);
+  a.by_page = fast_div(a.page);
 }
 
 void launch_paged_attention(const PagedAttnArgs& a, DecodeType t, hipStream_t stream) {
