@@ -40,7 +40,7 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 32;       // tokens a wave takes at a time
-constexpr int kMaxSplit = 128;  // parts of a sequence
+constexpr int kMaxSplit = 64;   // parts of a sequence
 
 template <DecodeType T>
 struct Elem;
@@ -76,17 +76,12 @@ struct Elem<kF32> {
   static __device__ __forceinline__ t store(float f) { return f; }
 };
 
-// waves of a workgroup where there are few workgroups: as many as leave each
-// the registers of two tiles (1,024 / 512 threads: 128 / 256 a lane)
-constexpr int many_waves(int type, int dim) {
-  const int row = dim * (type == kF32 ? 4 : 2);
-  return row <= 128 ? 16 : row <= 256 ? 8 : 4;
-}
-
-// waves a SIMD holds at least of a 4-wave workgroup's kernel
+// Waves a SIMD holds at least, by a token's row in bytes.  Many waves with one
+// tile each in flight beat fewer that load the next tile under the products:
+// 64 x 12 heads of 64 bf16, up to 1,024 tokens, 27.3 against 29.6 us.
 constexpr int min_waves(int type, int dim) {
   const int row = dim * (type == kF32 ? 4 : 2);
-  return row <= 64 ? 4 : row <= 128 ? 3 : row <= 256 ? 2 : 1;
+  return row <= 128 ? 4 : row <= 256 ? 3 : 1;
 }
 
 // what a lane holds of 32 tokens: dwords of K rows and of V columns
@@ -107,7 +102,7 @@ __device__ __forceinline__ int v_col(int m, int j) {
 }
 
 template <DecodeType T, int HD, int W>
-__global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) paged_attn_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(PagedAttnArgs a) {
   typedef Elem<T> E;
   typedef typename E::t S;
   typedef Tile<T, HD> Regs;
@@ -303,23 +298,11 @@ __global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) page
   const int t0 = sp * per + w;
   if (t0 < t_end) {
     int ids = a.split == 1 ? sound(t0 * kTile + (lane & 31) <= last ? early : 0) : look(t0);
-    if constexpr (HD * EB <= 512) {  // the next tile's loads run under this one's products
-      Regs cur, nxt;
-      for (int t = t0; t < t_end + W; t += W) {  // (one copy of each: the code, too, has to be read)
-        if (t < t_end) {
-          load(t, ids, nxt);
-          if (t + W < t_end) ids = look(t + W);
-        }
-        if (t > t0) compute(t - W, cur);
-        cur = nxt;
-      }
-    } else {
-      for (int t = t0; t < t_end; t += W) {
-        Regs cur;
-        load(t, ids, cur);
-        if (t + W < t_end) ids = look(t + W);
-        compute(t, cur);
-      }
+    for (int t = t0; t < t_end; t += W) {
+      Regs r;
+      load(t, ids, r);
+      if (t + W < t_end) ids = look(t + W);  // (under this tile's loads)
+      compute(t, r);
     }
   }
 
@@ -378,7 +361,7 @@ __global__ void __launch_bounds__(W * 64, W > 4 ? W / 4 : min_waves(T, HD)) page
 template <DecodeType T>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnArgs a) {
   typedef Elem<T> E;
-  __shared__ float s_w[kMaxSplit], s_num[256], s_top[4], s_den[4];
+  __shared__ float s_w[256], s_num[256], s_top[4], s_den[4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int at = blockIdx.x, n = a.by_heads.of(at);
   const int len = a.lens[n];
@@ -397,7 +380,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnArgs a) {
   __syncthreads();
   m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
   const float f = exp2f(top - m);
-  if (tid < kMaxSplit) s_w[tid] = f;
+  s_w[tid] = f;
   den *= f;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
@@ -436,9 +419,8 @@ void launch_one(const PagedAttnArgs& a, hipStream_t stream) {
 
 template <DecodeType T, int HD>
 void launch_dim(const PagedAttnArgs& a, hipStream_t stream) {
-  constexpr int kMany = many_waves(T, HD);
-  if constexpr (kMany > 4) {
-    if (a.waves == kMany) return launch_one<T, HD, kMany>(a, stream);
+  if constexpr (HD * Tile<T, HD>::E <= 256) {
+    if (a.waves == 8) return launch_one<T, HD, 8>(a, stream);
   }
   launch_one<T, HD, 4>(a, stream);
 }
@@ -453,14 +435,21 @@ void launch_type(const PagedAttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// Waves a workgroup and parts a sequence: a workgroup serves one (sequence,
-// cache head, 16 query heads), its waves take the sequence's tiles in turn.
+// Waves a workgroup and parts a sequence.  A workgroup serves one (sequence,
+// cache head, 16 query heads), its waves take the sequence's tiles in turn: 8
+// of them, 4 where sequences are short (one or two tiles a wave: 64 x 12 heads
+// of up to 256 tokens 10.7 against 12.0 us) or rows fill the registers.  Where
+// there are fewer than 1,024 workgroups, a sequence of 6 or more tiles a wave
+// is split so that two are left: 1 x 12 heads, 4,096 tokens 11.5 against 29.7
+// us, 8 x 8 heads, 65,536 tokens 245 against 776; below that the second launch
+// costs more than it saves (16 x 12 heads, 1,024 tokens 15.5 against 11.9).
 void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest) {
-  const int group = a.heads / a.kv_heads, cols = group < 16 ? group : 16;
+  const int group = a.heads / a.kv_heads;
   const int64_t groups = static_cast<int64_t>(a.n) * a.kv_heads * ((group + 15) / 16);
   const int64_t tiles = (longest + kTile - 1) / kTile;
-  a.waves = groups < 512 && cols * a.dim <= 1024 ? many_waves(t, a.dim) : 4;
-  int64_t split = (512 + groups - 1) / (groups > 0 ? groups : 1);
+  a.waves = tiles > 8 && a.dim * (t == kF32 ? 4 : 2) <= 256 ? 8 : 4;
+  int64_t split = 1;
+  if (groups > 0 && tiles >= 6 * a.waves) split = (1024 + groups - 1) / groups;
   const int64_t most = tiles / (2 * a.waves);
   split = split > most ? most : split;
   a.split = static_cast<int>(split < 1 ? 1 : split > kMaxSplit ? kMaxSplit : split);
