@@ -9,7 +9,8 @@
 //
 // Two launches, bound by reading the logits once.  Within a row a score is
 // monotone in the logit, so the first kernel ranks raw logits and never forms
-// a score: a workgroup holds up to 8,192 of a row's logits in registers, takes
+// a score: a workgroup holds up to 16,384 of a row's logits (8,192
+// in fp32) in registers, takes
 // their maximum, the sum of exponentials beside it and the `keep` best of
 // them.  The second turns what is left of a request (beams x parts x keep)
 // into scores, in 64 bits: candidates of different beams may lie closer than
@@ -19,9 +20,10 @@
 // hold an element that is no less than the keep-th largest of the lanes' own
 // maxima, so nothing below that (the largest such of the waves) can be among
 // the `keep` best.  It is found by bits with a ballot a bit, some 2 keep to 4
-// keep elements pass, and those are ranked by counting.  Where more than kList
-// pass (thousands of equal logits) `keep` rounds of an argmax take over.
+// keep elements pass, and those are ranked by counting.  Where more than the
+// lists hold pass (thousands of equal logits) `keep` rounds of an argmax take over.
 #include <hip/hip_runtime.h>
+#include <cfloat>
 #include <cstdint>
 #include "conv_common.h"
 #include "decode.h"
@@ -30,8 +32,11 @@ namespace commeff {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRow = 32;     // logits a thread holds
-constexpr int kList = 1024;  // candidates that are ranked by counting
+constexpr int kPieces = 8;   // 16-byte pieces of a row that a thread holds
+constexpr int kList = 256;   // candidates of a wave that are ranked by counting
+constexpr int kJoinList = 1024;  // .. of the join
+
+constexpr float kLog2e = 1.44269504088896340736f;
 
 typedef unsigned long long u64;
 
@@ -41,6 +46,9 @@ __device__ __forceinline__ float to_float(uint32_t bits) {  // of one element
   else if constexpr (T == kF16) return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
   else return __uint_as_float(bits);
 }
+
+template <DecodeType T>
+constexpr uint32_t kLow = T == kBf16 ? 0xff80ff80u : T == kF16 ? 0xfc00fc00u : 0xff800000u;  // -inf
 
 // unsigned integers in the order of the floats (+0 and -0 made one before)
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -60,7 +68,8 @@ __device__ __forceinline__ double unordered(u64 u) {
 constexpr uint32_t kNone = 0x007fffffu;  // ordered(-inf): no candidate
 
 // a bound that at least `keep` lanes' values reach (0 where fewer than `keep`
-// lanes have any): the keep-th largest, or less by bits that do not matter
+// lanes have any): the keep-th largest, or less by bits that do not matter;
+// two bits at a time, since a ballot's way to the next comparison is what costs
 __device__ __forceinline__ uint32_t wave_bound(uint32_t x, int keep) {
   uint32_t bound = 0;
   for (int bit = 31; bit >= 0; --bit) {
@@ -100,109 +109,140 @@ __device__ __forceinline__ Best block_best(Best x, Best* lds) {
 // their order, 0 where there are fewer
 template <DecodeType T>
 __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
-  constexpr int EB = T == kF32 ? 4 : 2, GE = 16 / EB, GT = kRow / GE;  // elements of 16 bytes, those of a thread
+  constexpr int EB = T == kF32 ? 4 : 2, GE = 16 / EB;  // elements of 16 bytes
   __shared__ float s_f[4];
   __shared__ double s_d[4];
   __shared__ uint32_t s_u[4];
-  __shared__ u64 s_list[kList];
+  __shared__ u64 s_list[4][kList];
   __shared__ Best s_best[4];
-  __shared__ int s_n;
+  __shared__ int s_n[4];
   const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const float score = a.scores[row];
   if ((a.finished && a.finished[row]) || !(fabsf(score) < INFINITY)) return;  // the logits do not matter
+  const int64_t req = a.by_beams.of(row);
   const unsigned char* p = static_cast<const unsigned char*>(a.logits) +
-                           (row / a.beams * a.s_request + row % a.beams * a.s_beam) * EB;
+                           (req * a.s_request + (row - req * a.beams) * a.s_beam) * EB;
   // 16-byte pieces counted from the multiple of 16 at or before the row's start
   const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / EB;
   const int pieces = (skew + a.vocab + GE - 1) / GE;
-  const int per = (pieces + a.parts - 1) / a.parts, end = min(pieces, (part + 1) * per);
-  float x[kRow];
+  const int per = a.by_parts.of(pieces + a.parts - 1), end = min(pieces, (part + 1) * per);
+  v4u u[kPieces];
 #pragma unroll
-  for (int i = 0; i < GT; ++i) {
+  for (int i = 0; i < kPieces; ++i) {
     const int pc = part * per + i * kThreads + tid;
     const int v0 = pc * GE - skew;
+    u[i] = v4u{kLow<T>, kLow<T>, kLow<T>, kLow<T>};
     if (pc < end && v0 >= 0 && v0 + GE <= a.vocab) {
-      const v4u u = *reinterpret_cast<const v4u*>(p + static_cast<int64_t>(v0) * EB);
+      u[i] = *reinterpret_cast<const v4u*>(p + static_cast<int64_t>(v0) * EB);
+    } else if (pc < end) {  // the row's ends: element by element
 #pragma unroll
       for (int e = 0; e < GE; ++e)
-        x[i * GE + e] = to_float<T>(EB == 4 ? u[e % 4] : (u[e / 2] >> (16 * (e & 1))) & 0xffffu);
-    } else {
-#pragma unroll
-      for (int e = 0; e < GE; ++e) {
-        x[i * GE + e] = -INFINITY;
-        if (pc < end && v0 + e >= 0 && v0 + e < a.vocab) {
-          if constexpr (EB == 4) x[i * GE + e] = reinterpret_cast<const float*>(p)[v0 + e];
-          else x[i * GE + e] = to_float<T>(reinterpret_cast<const uint16_t*>(p)[v0 + e]);
+        if (v0 + e >= 0 && v0 + e < a.vocab) {
+          if constexpr (EB == 4) u[i][e] = reinterpret_cast<const uint32_t*>(p)[v0 + e];
+          else u[i][e / 2] = (u[i][e / 2] & (0xffffu << (16 * (1 - (e & 1))))) |
+                             static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[v0 + e]) << (16 * (e & 1));
         }
-      }
     }
   }
+  auto at = [&](int i, int e) {  // element e of piece i
+    return to_float<T>(EB == 4 ? u[i][e % 4] : (u[i][e / 2] >> (16 * (e & 1))) & 0xffffu);
+  };
+  float top[kPieces];
   float most = -INFINITY;
-  bool odd = false;
 #pragma unroll
-  for (int i = 0; i < kRow; ++i) {
-    x[i] += 0.f;  // -0 is +0
-    odd |= !(x[i] < INFINITY);
-    most = fmaxf(most, x[i]);
+  for (int i = 0; i < kPieces; ++i) {
+    top[i] = at(i, 0);
+#pragma unroll
+    for (int e = 1; e < GE; ++e) top[i] = fmaxf(top[i], at(i, e));
+    most = fmaxf(most, top[i]);
   }
-  uint32_t bound = wave_bound(ordered(most), a.keep);
+  // (unpacked again for each use: held, the numbers would cost half the waves)
+  auto anew = [&] {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) asm volatile("" : "+v"(u[i]));
+  };
+  anew();
+  uint32_t bound = wave_bound(ordered(most + 0.f), a.keep);
   float m = most;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (__any(odd)) m = INFINITY;
-  if (lane == 0) s_f[w] = m, s_u[w] = bound;
-  if (tid == 0) s_n = 0;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_f[0], s_f[1]), fmaxf(s_f[2], s_f[3]));
-  bound = max(max(max(s_u[0], s_u[1]), max(s_u[2], s_u[3])), kNone + 1);
-  double* stat = a.stat + (static_cast<int64_t>(row) * a.parts + part) * 2;
-  u64* cand = a.cand + (static_cast<int64_t>(row) * a.parts + part) * a.keep;
-  if (!(fabsf(m) < INFINITY)) {  // nothing above -inf, or no row at all
-    if (tid == 0) stat[0] = m, stat[1] = 0.0;
-    for (int k = tid; k < a.keep; k += kThreads) cand[k] = 0;
-    return;
-  }
-  // the difference first: its rounding is that of a small number
+  // the exponentials beside the wave's own maximum; the difference first, so
+  // that its rounding is that of a small number.  NaN (+inf - inf too) stays.
+  const float beside = fmaxf(m, -FLT_MAX);
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kRow; ++i) sum += __builtin_amdgcn_exp2f((x[i] - m) * 1.44269504088896340736f);
+  for (int i = 0; i < kPieces; ++i)
+    if (i * kThreads < per) {  // (a whole piece of the workgroup: rows shorter than its registers)
+#pragma unroll
+      for (int e = 0; e < GE; ++e) sum += __builtin_amdgcn_exp2f((at(i, e) - beside) * kLog2e);
+    }
   double all = sum;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, 64);
-  if (lane == 0) s_d[w] = all;
-  auto key = [&](int i) {
-    const int v = (part * per + i / GE * kThreads + tid) * GE - skew + i % GE;
-    return static_cast<u64>(ordered(x[i])) << 32 | (0xffffffffu - static_cast<uint32_t>(v));
-  };
-  if (ordered(most) >= bound) {
-#pragma unroll
-    for (int i = 0; i < kRow; ++i)
-      if (ordered(x[i]) >= bound) {
-        const int at = atomicAdd(&s_n, 1);  // (any order: the list is ranked)
-        if (at < kList) s_list[at] = key(i);
-      }
-  }
+  if (lane == 0) s_f[w] = m, s_u[w] = bound, s_d[w] = all;
   __syncthreads();
-  if (tid == 0) stat[0] = m, stat[1] = s_d[0] + s_d[1] + s_d[2] + s_d[3];
-  const int n = s_n;
-  if (n <= kList) {
-    for (int c = tid; c < n; c += kThreads) {
-      const u64 mine = s_list[c];
+  m = fmaxf(fmaxf(s_f[0], s_f[1]), fmaxf(s_f[2], s_f[3]));
+  bound = max(max(max(s_u[0], s_u[1]), max(s_u[2], s_u[3])), kNone + 1);
+  all = 0.0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i)
+    all += s_d[i] * __builtin_amdgcn_exp2f((fmaxf(s_f[i], -FLT_MAX) - fmaxf(m, -FLT_MAX)) * kLog2e);
+  double* stat = a.stat + (static_cast<int64_t>(row) * a.parts + part) * 2;
+  u64* cand = a.cand + (static_cast<int64_t>(row) * a.parts + part) * a.keep;
+  if (!(fabsf(m) < INFINITY) || all != all) {  // nothing above -inf, or no row at all
+    if (tid == 0) stat[0] = all != all ? INFINITY : m, stat[1] = 0.0;
+    for (int k = tid; k < a.keep; k += kThreads) cand[k] = 0;
+    return;
+  }
+  if (tid == 0) stat[0] = m, stat[1] = all;
+  auto key = [](float x, int v) {  // (-0 is +0)
+    return static_cast<u64>(ordered(x + 0.f)) << 32 | (0xffffffffu - static_cast<uint32_t>(v));
+  };
+  anew();
+  const float least = unordered(bound);  // (from -FLT_MAX on: a number)
+  int mine = 0;  // of the wave's list
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i)
+    if (__any(top[i] >= least)) {
+#pragma unroll
+      for (int e = 0; e < GE; ++e) {
+        const bool in = at(i, e) >= least;
+        const u64 mask = __ballot(in);
+        if (mask == 0) continue;
+        const int c = mine + __popcll(mask & ((1ull << lane) - 1));
+        if (in && c < kList) s_list[w][c] = key(at(i, e), (part * per + i * kThreads + tid) * GE - skew + e);
+        mine += __popcll(mask);
+      }
+    }
+  if (lane == 0) s_n[w] = mine;
+  __syncthreads();
+  const int most_n = max(max(s_n[0], s_n[1]), max(s_n[2], s_n[3])), n = s_n[0] + s_n[1] + s_n[2] + s_n[3];
+  if (most_n <= kList) {
+    // a wave ranks its own list, four lanes a candidate, each against one list
+    const int q = lane & 3, nq = s_n[q];
+    for (int c = lane >> 2; c < mine; c += 16) {
+      const u64 k = s_list[w][c];
       int rank = 0;
-      for (int i = 0; i < n; ++i) rank += s_list[i] > mine;
-      if (rank < a.keep) cand[rank] = mine;
+#pragma unroll 4
+      for (int i = 0; i < nq; ++i) rank += s_list[q][i] > k;
+      rank += __shfl_xor(rank, 1, 64);
+      rank += __shfl_xor(rank, 2, 64);
+      if (q == 0 && rank < a.keep) cand[rank] = k;
     }
     for (int k = n + tid; k < a.keep; k += kThreads) cand[k] = 0;
     return;
   }
-  u64 last = ~0ull;
+  u64 last = ~0ull;  // (the row again from the cache: rare, and no registers for it)
   for (int k = 0; k < a.keep; ++k) {
     Best b = {0, 0};
-#pragma unroll
-    for (int i = 0; i < kRow; ++i) {
-      const u64 c = key(i);
-      if (ordered(x[i]) > kNone && c < last && c > b.value) b.value = c;
-    }
+    for (int pc = part * per + tid; pc < end; pc += kThreads)
+      for (int v = max(pc * GE - skew, 0); v < min((pc + 1) * GE - skew, a.vocab); ++v) {
+        float x;
+        if constexpr (EB == 4) x = reinterpret_cast<const float*>(p)[v];
+        else x = to_float<T>(reinterpret_cast<const uint16_t*>(p)[v]);
+        const u64 c = key(x, v);
+        if (x > -INFINITY && c < last && c > b.value) b.value = c;
+      }
     b = block_best(b, s_best);
     last = b.value;
     if (tid == 0) cand[k] = last;
@@ -210,9 +250,11 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
 }
 
 // a request's beams: their log-sum-exp, the scores of what the parts kept, and
-// the best of them
+// the best of them.  Bound by latency: the first candidates are on their way
+// while the sums are joined (a wave a beam), and stay in registers.
 __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
-  __shared__ Best s_list[kList];
+  constexpr int kHeld = 4;  // candidates a thread holds
+  __shared__ Best s_list[kJoinList];
   __shared__ Best s_best[4];
   __shared__ uint32_t s_u[4];
   __shared__ int s_n;
@@ -220,67 +262,94 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t row0 = static_cast<int64_t>(b) * a.beams;
   auto ends = [&](int j) { return a.finished && a.finished[row0 + j]; };
-  for (int j = tid; j < a.beams; j += kThreads) {
-    const double* stat = a.stat + (row0 + j) * a.parts * 2;
+  auto alive = [&](int j) { return !ends(j) && fabsf(a.scores[row0 + j]) < INFINITY; };
+  // candidate c: the (c / lists)-th of list c % lists, so that a wave's lanes see the lists' heads
+  const int lists = a.beams * a.parts, all = lists * a.keep;
+  auto place = [&](int c, int& rank, int& list, int& j) {
+    rank = a.by_lists.of(c);
+    list = c - rank * lists;
+    j = a.by_parts.of(list);
+  };
+  auto fetch = [&](int c) {
+    int rank, list, j;
+    place(c, rank, list, j);
+    return a.cand[(row0 * a.parts + list) * a.keep + rank];  // (of a beam that has none: not looked at)
+  };
+  u64 held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = tid + i * kThreads < all ? fetch(tid + i * kThreads) : 0;
+  for (int j = w; j < a.beams; j += kThreads / 64) {
     double lse = INFINITY;
-    if (!ends(j) && fabsf(a.scores[row0 + j]) < INFINITY) {
-      double m = -INFINITY;
-      for (int i = 0; i < a.parts; ++i) m = fmax(m, stat[2 * i]);
+    const double* stat = a.stat + (row0 + j) * a.parts * 2;
+    double m = -INFINITY, sum = 0.0;
+    for (int i = lane; i < a.parts; i += 64) m = fmax(m, stat[2 * i]);
+    if (alive(j)) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
       if (fabs(m) < INFINITY) {
-        double sum = 0.0;
-        for (int i = 0; i < a.parts; ++i) sum += stat[2 * i + 1] * exp(stat[2 * i] - m);
+        for (int i = lane; i < a.parts; i += 64)
+          if (stat[2 * i + 1] > 0.0) sum += stat[2 * i + 1] * exp(stat[2 * i] - m);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         lse = m + log(sum);
       }
     }
-    s_lse[j] = lse;
+    if (lane == 0) s_lse[j] = lse;
   }
   if (tid == 0) s_n = 0;
   __syncthreads();
-  const int per = a.parts * a.keep;
-  const int64_t all = static_cast<int64_t>(a.beams) * per;
-  // candidate c: the (c / lists)-th of list c % lists, so that a wave's lanes see the lists' heads
-  const int lists = a.beams * a.parts;
-  auto score = [&](int64_t c) {  // value 0: none
-    const int rank = static_cast<int>(c / lists), list = static_cast<int>(c - static_cast<int64_t>(rank) * lists);
-    const int j = list / a.parts, part = list - j * a.parts;
+  auto score = [&](int c, u64 k) {  // value 0: none
+    int rank, list, j;
+    place(c, rank, list, j);
     const double s = a.scores[row0 + j];
     if (ends(j)) {
-      if (rank != 0 || part != 0 || !(fabs(s) < INFINITY)) return Best{0, 0};
+      if (rank != 0 || list != j * a.parts || !(fabs(s) < INFINITY)) return Best{0, 0};
       return Best{ordered(s + 0.0), static_cast<u64>(j) * a.vocab + a.eos};
     }
-    if (s_lse[j] == INFINITY) return Best{0, 0};
-    const u64 k = a.cand[(row0 + j) * per + part * a.keep + rank];
-    if (k == 0) return Best{0, 0};
+    if (k == 0 || s_lse[j] == INFINITY) return Best{0, 0};
     const double x = s + (unordered(static_cast<uint32_t>(k >> 32)) - s_lse[j]);
     return Best{ordered(x + 0.0), static_cast<u64>(j) * a.vocab + (0xffffffffu - static_cast<uint32_t>(k))};
   };
+  Best mine[kHeld];
   uint32_t most = 0;  // the upper halves do for a bound
-  for (int64_t c = tid; c < all; c += kThreads) most = max(most, static_cast<uint32_t>(score(c).value >> 32));
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    mine[i] = tid + i * kThreads < all ? score(tid + i * kThreads, held[i]) : Best{0, 0};
+    most = max(most, static_cast<uint32_t>(mine[i].value >> 32));
+  }
+  for (int c = tid + kHeld * kThreads; c < all; c += kThreads)
+    most = max(most, static_cast<uint32_t>(score(c, fetch(c)).value >> 32));
   uint32_t bound = wave_bound(most, a.keep);
   if (lane == 0) s_u[w] = bound;
   __syncthreads();
   bound = max(max(s_u[0], s_u[1]), max(max(s_u[2], s_u[3]), 1u));
-  for (int64_t c = tid; c < all; c += kThreads) {
-    const Best x = score(c);
+  auto pass = [&](const Best& x) {
     if (static_cast<uint32_t>(x.value >> 32) >= bound) {
       const int at = atomicAdd(&s_n, 1);  // (any order: the list is ranked)
-      if (at < kList) s_list[at] = x;
+      if (at < kJoinList) s_list[at] = x;
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) pass(mine[i]);
+  for (int c = tid + kHeld * kThreads; c < all; c += kThreads) pass(score(c, fetch(c)));
   __syncthreads();
   const int n = s_n;
   auto put = [&](int k, const Best& x, bool some) {
     const int64_t at = static_cast<int64_t>(b) * a.keep + k;
+    const int j = some ? static_cast<int>(x.index) / a.vocab : 0;  // (beams x vocabulary < 2^31)
     a.out_scores[at] = some ? static_cast<float>(unordered(x.value)) : -INFINITY;
-    a.out_parent[at] = some ? static_cast<int64_t>(x.index / a.vocab) : 0;
-    a.out_token[at] = some ? static_cast<int64_t>(x.index % a.vocab) : 0;
+    a.out_parent[at] = j;
+    a.out_token[at] = some ? static_cast<int>(x.index) - j * a.vocab : 0;
   };
-  if (n <= kList) {
-    for (int c = tid; c < n; c += kThreads) {
-      const Best mine = s_list[c];
+  if (n <= kJoinList) {
+    for (int c = tid >> 2; c < n; c += kThreads / 4) {
+      const Best x = s_list[c];
       int rank = 0;
-      for (int i = 0; i < n; ++i) rank += before(s_list[i], mine);
-      if (rank < a.keep) put(rank, mine, true);
+#pragma unroll 4
+      for (int i = tid & 3; i < n; i += 4) rank += before(s_list[i], x);
+      rank += __shfl_xor(rank, 1, 64);
+      rank += __shfl_xor(rank, 2, 64);
+      if ((tid & 3) == 0 && rank < a.keep) put(rank, x, true);
     }
     for (int k = n + tid; k < a.keep; k += kThreads) put(k, Best{0, 0}, false);
     return;
@@ -288,8 +357,8 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   Best last = {~0ull, 0};
   for (int k = 0; k < a.keep; ++k) {
     Best x = {0, ~0ull};
-    for (int64_t c = tid; c < all; c += kThreads) {
-      const Best y = score(c);
+    for (int c = tid; c < all; c += kThreads) {
+      const Best y = score(c, fetch(c));
       if (before(last, y) && before(y, x)) x = y;
     }
     x = block_best(x, s_best);
@@ -306,14 +375,17 @@ void launch_type(const BeamSelectArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// equal parts of at most 8,192 logits, whatever the row's alignment adds
+// equal parts of at most 2,048 pieces, whatever the row's alignment adds
 int beam_select_parts(int vocab, DecodeType t) {
-  const int ge = t == kF32 ? 4 : 8, most = kThreads * kRow / ge;
+  const int ge = t == kF32 ? 4 : 8, most = kThreads * kPieces;
   return ((vocab + ge - 1) / ge + 1 + most - 1) / most;
 }
 
-void launch_beam_select(const BeamSelectArgs& a, DecodeType t, hipStream_t stream) {
+void launch_beam_select(BeamSelectArgs a, DecodeType t, hipStream_t stream) {
   if (a.requests == 0) return;
+  a.by_beams = fast_div(a.beams);
+  a.by_parts = fast_div(a.parts);
+  a.by_lists = fast_div(static_cast<int64_t>(a.beams) * a.parts);
   if (t == kBf16) launch_type<kBf16>(a, stream);
   else if (t == kF16) launch_type<kF16>(a, stream);
   else launch_type<kF32>(a, stream);

@@ -49,8 +49,10 @@ struct KvExtendArgs {
   int32_t* start;        // [n + 1]
   int32_t* missed;       // [1]
   int32_t *lens_out, *used_out;  // may be lens / used
-  int32_t *base, *first;         // scratch [n]: length before, or -1; first pool index
+  int32_t *base, *first;         // scratch [n] unless fused: length before, or -1; first pool index
   int n, width, page, rows, pool_n;
+  int search, wide;  // launch_kv_extend: the first step of a search, 16-byte loads
+  FastDiv by_page;
 };
 
 struct KvWriteArgs {
@@ -62,6 +64,8 @@ struct KvWriteArgs {
   int64_t rows, pages;
   int heads, page, row_bytes;  // row_bytes: one head's
   int unit;                    // bytes moved at once: 16, 4 or 2
+  int chunk;                   // launch_kv_write
+  FastDiv by_unit, by_heads, by_page;
 };
 
 struct BeamReorderArgs {
@@ -73,6 +77,7 @@ struct BeamReorderArgs {
   int64_t s_layer, s_kv, s_page, s_head, s_tok;  // bytes
   int64_t pages;
   int requests, beams, width, layers, heads, page, row_bytes, unit;
+  FastDiv by_page, by_heads, by_unit;  // launch_beam_reorder
 };
 
 struct PagedAttnArgs {
@@ -103,15 +108,17 @@ struct BeamSelectArgs {
   int64_t s_request, s_beam;  // elements
   int64_t eos;
   int requests, beams, vocab, keep, parts;
+  FastDiv by_beams, by_parts, by_lists;  // launch_beam_select
 };
 
-void launch_kv_extend(const KvExtendArgs& a, hipStream_t stream);
-void launch_kv_write(const KvWriteArgs& a, hipStream_t stream);
-void launch_beam_reorder(const BeamReorderArgs& a, hipStream_t stream);
+bool kv_extend_fused(const KvExtendArgs& a);  // one launch, the plan in LDS
+void launch_kv_extend(KvExtendArgs a, hipStream_t stream);
+void launch_kv_write(KvWriteArgs a, hipStream_t stream);
+void launch_beam_reorder(BeamReorderArgs a, hipStream_t stream);
 void launch_paged_attention(const PagedAttnArgs& a, DecodeType t, hipStream_t stream);
 // fills in the split and the divisors; longest: a hint of the longest sequence
 void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest);
-void launch_beam_select(const BeamSelectArgs& a, DecodeType t, hipStream_t stream);
+void launch_beam_select(BeamSelectArgs a, DecodeType t, hipStream_t stream);
 int beam_select_parts(int vocab, DecodeType t);
 
 }  // namespace commeff

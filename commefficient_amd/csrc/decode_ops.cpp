@@ -120,17 +120,26 @@ std::vector<at::Tensor> extend_outputs(at::Tensor& table, at::Tensor& lens, cons
   TORCH_CHECK(rows >= 0 && rows <= (1ll << 30), op, ": rows must be in [0, 2^30], not ", rows);
   TORCH_CHECK(n <= (1ll << 30) && pool.numel() <= (1ll << 30), op, ": at most 2^30 sequences and pages");
   auto i32 = lens.options();
-  // one allocation: pos [rows] | seq [rows] | start [n + 1] | missed | lens [n] | used
-  const int64_t own = in_place ? 0 : n + 1;
-  auto buf = at::empty({2 * rows + n + 2 + own}, i32);
-  std::vector<at::Tensor> out{at::empty({rows}, i32.dtype(at::kLong)), buf.narrow(0, 0, rows),
-                              buf.narrow(0, rows, rows), buf.narrow(0, 2 * rows, n + 1),
-                              buf.narrow(0, 2 * rows + n + 1, 1)};
+  // slots [rows] | one allocation: pos [rows], seq [rows], start [n + 1], missed (, lens [n], used)
+  const int64_t all = 2 * rows + n + 2 + (in_place ? 0 : n + 1);
+  const auto buf = at::empty({all}, i32);
+  int64_t at = 0;
+  auto piece = [&](int64_t size) {  // (a narrow() without the dispatcher: half of this call's host time otherwise)
+    auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+    t->set_storage_offset(at);
+    t->set_sizes_contiguous({size});
+    at += size;
+    return at::Tensor(std::move(t));
+  };
+  std::vector<at::Tensor> out;
+  out.reserve(7);
+  out.push_back(at::empty({rows}, i32.dtype(at::kLong)));
+  for (int64_t size : {rows, rows, n + 1, static_cast<int64_t>(1)}) out.push_back(piece(size));
   if (!in_place) {
-    out.push_back(buf.narrow(0, 2 * rows + n + 2, n));
-    out.push_back(buf.narrow(0, 2 * rows + 2 * n + 2, 1));
+    out.push_back(piece(n));
+    out.push_back(piece(1));
   }
-  return out;  // slots, pos, seq, start, missed (, lens, used)
+  return out;
 }
 
 std::vector<at::Tensor> kv_extend_hip(at::Tensor table, at::Tensor lens, const at::Tensor& fresh,
@@ -139,7 +148,7 @@ std::vector<at::Tensor> kv_extend_hip(at::Tensor table, at::Tensor lens, const a
   c10::hip::HIPGuardMasqueradingAsCUDA guard(table.device());
   auto out = extend_outputs(table, lens, fresh, pool, used, page, rows, in_place);
   const int64_t n = table.size(0);
-  auto work = at::empty({2 * n}, lens.options());
+  at::Tensor work;
   KvExtendArgs a;
   a.table = table.data_ptr<int32_t>();
   a.table_ld = table.stride(0);
@@ -154,13 +163,17 @@ std::vector<at::Tensor> kv_extend_hip(at::Tensor table, at::Tensor lens, const a
   a.missed = out[4].data_ptr<int32_t>();
   a.lens_out = (in_place ? lens : out[5]).data_ptr<int32_t>();
   a.used_out = (in_place ? used : out[6]).data_ptr<int32_t>();
-  a.base = work.data_ptr<int32_t>();
-  a.first = a.base + n;
+  a.base = a.first = nullptr;
   a.n = static_cast<int>(n);
   a.width = static_cast<int>(table.size(1));
   a.page = static_cast<int>(page);
   a.rows = static_cast<int>(rows);
   a.pool_n = static_cast<int>(pool.numel());
+  if (!kv_extend_fused(a)) {
+    work = at::empty({2 * n}, lens.options());
+    a.base = work.data_ptr<int32_t>();
+    a.first = a.base + n;
+  }
   launch_kv_extend(a, stream_now());
   return out;
 }
@@ -216,7 +229,12 @@ void check_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc,
   const char* op = "kv_write";
   decode_type(kc, op, "the key cache");
   check_pair(kc, vc, op);
+  check_page(kc.size(2), 0, op);
+  TORCH_CHECK(kc.size(0) * kc.size(2) < (1ll << 31), op, ": the caches must hold less than 2^31 slots, not ",
+              kc.size(0), " pages of ", kc.size(2));
   check_rows(k, -1, kc, op, "k");
+  TORCH_CHECK(k.size(0) < (1ll << 31) && k.size(1) * k.size(2) <= (1ll << 24), op, ": rows too many or too long: ",
+              k.sizes());
   check_rows(v, k.size(0), vc, op, "v");
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
                   slots.numel() == k.size(0),
@@ -269,6 +287,7 @@ void check_reorder(const at::Tensor& parent, const at::Tensor& table, const at::
                   parent.numel() == table.size(0),
               op, ": parent must be contiguous int64 [requests, beams] over the table's ", table.size(0),
               " sequences, not ", parent.scalar_type(), " ", parent.sizes());
+  TORCH_CHECK(parent.size(0) <= 65535, op, ": at most 65,535 requests, not ", parent.size(0));
   TORCH_CHECK(parent.size(1) <= kReorderMaxBeams, op, ": at most ", kReorderMaxBeams, " beams, not ", parent.size(1));
   same_device(parent, table, op, "parent");
   check_i32(lens, table.size(0), table, op, "lens");
@@ -281,6 +300,8 @@ void check_reorder(const at::Tensor& parent, const at::Tensor& table, const at::
     TORCH_CHECK(kv.size(d) <= 1 || kv.stride(d) > 0, op, ": kv is an expanded view");
   same_device(kv, table, op, "kv");
   check_page(kv.size(4), table.size(1), op);
+  TORCH_CHECK(2 * kv.size(0) * kv.size(3) * kv.size(4) * kv.size(5) < (1ll << 31), op,
+              ": a page of all layers holds less than 2^31 numbers, not ", kv.sizes());
 }
 
 void beam_reorder_hip(const at::Tensor& parent, at::Tensor table, const at::Tensor& lens, at::Tensor kv) {
@@ -535,6 +556,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_hip(const at::Tensor&
   const DecodeType type = decode_type(x, "beam_select", "logits");
   a.parts = beam_select_parts(a.vocab, type);
   const int64_t lists = scores.numel() * a.parts;
+  TORCH_CHECK(x.size(1) * a.parts * keep < (1ll << 31), "beam_select: too many beams for this vocabulary");
   auto work = at::empty({lists * (keep + 2)}, scores.options().dtype(at::kLong));
   a.cand = reinterpret_cast<unsigned long long*>(work.data_ptr<int64_t>());
   a.stat = reinterpret_cast<double*>(a.cand + lists * keep);

@@ -24,7 +24,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 constexpr int kScan = 1024, kEach = 4;  // threads of the scan, sequences a thread takes at once
 constexpr int kFused = 8192;            // sequences and rows of a single launch
 
-// inclusive scan of min(a + b, cap) over the block, values <= cap <= 2^30 + 1;
+// exclusive scan of min(a + b, cap) over the block, values <= cap <= 2^30 + 1;
 // `total`: all of it
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t cap, uint32_t* lds, uint32_t* total) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -43,43 +43,59 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t cap, uint32_
     all = min(all + lds[i], cap);
   }
   *total = all;
-  return min(before + v, cap);
+  v = __shfl_up(v, 1, 64);
+  return lane == 0 ? before : min(before + v, cap);
 }
 
 struct KvPlan {  // of the sequences: LDS, or global memory
   int32_t *start, *base, *first;
 };
 
-// row r: its slot, position and sequence, and the table entry where it opens a page
-__device__ __forceinline__ void extend_row(const KvExtendArgs& a, const KvPlan& p, int r) {
-  int lo = 0, hi = a.n;  // the first sequence that ends past r
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (p.start[mid + 1] > r) hi = mid;
-    else lo = mid + 1;
-  }
-  int64_t slot = -1;
-  int pos = 0;
-  if (lo < a.n) {
-    const int len = p.base[lo];
+// rows r, r + step, ..: slot, position, sequence, and the table entry where one
+// opens a page.  ROWS searches, and then loads, of a thread run side by side.
+template <int ROWS>
+__device__ __forceinline__ void extend_rows(const KvExtendArgs& a, const KvPlan& p, int r0, int step) {
+  int seq[ROWS], pos[ROWS], off[ROWS];
+  const int32_t* src[ROWS];
+  int32_t* dst[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) seq[k] = 0;
+  // the sequences that end at or before the row: start[i] <= r for i <= that many
+  for (int s = a.search; s > 0; s >>= 1)
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      if (seq[k] + s <= a.n && p.start[seq[k] + s] <= r0 + k * step) seq[k] += s;
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const int i = seq[k], r = r0 + k * step;
+    const int len = i < a.n && r < a.rows ? p.base[i] : -1;
+    src[k] = nullptr;
+    dst[k] = nullptr;
+    pos[k] = off[k] = 0;
     if (len >= 0) {
-      pos = len + r - p.start[lo];
-      const int pi = static_cast<uint32_t>(pos) / static_cast<uint32_t>(a.page);
-      const int have = static_cast<uint32_t>(len + a.page - 1) / static_cast<uint32_t>(a.page);
-      int32_t* row = a.table + lo * a.table_ld;
-      int64_t id;
-      if (pi < have) {
-        id = row[pi];
-      } else {
-        id = a.pool[p.first[lo] + pi - have];
-        if (pos == pi * a.page) row[pi] = static_cast<int32_t>(id);
+      pos[k] = len + r - p.start[i];
+      const int pi = a.by_page.of(pos[k]), have = a.by_page.of(len + a.page - 1);
+      off[k] = pos[k] - pi * a.page;
+      int32_t* row = a.table + i * a.table_ld + pi;
+      src[k] = row;
+      if (pi >= have) {
+        src[k] = a.pool + p.first[i] + pi - have;
+        if (off[k] == 0) dst[k] = row;
       }
-      if (id >= 0) slot = id * a.page + (pos - pi * a.page);
     }
   }
-  a.slots[r] = slot;
-  a.pos[r] = pos;
-  a.seq[r] = lo < a.n ? lo : -1;
+  int id[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) id[k] = src[k] ? *src[k] : -1;
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const int r = r0 + k * step;
+    if (r >= a.rows) continue;
+    if (dst[k]) *dst[k] = id[k];
+    a.slots[r] = id[k] < 0 ? -1 : static_cast<int64_t>(id[k]) * a.page + off[k];
+    a.pos[r] = pos[k];
+    a.seq[r] = seq[k] < a.n ? seq[k] : -1;
+  }
 }
 
 template <bool FUSED>
@@ -93,7 +109,7 @@ __global__ void __launch_bounds__(kScan) kv_extend_kernel(KvExtendArgs a) {
   if (tid == 0) s_got = s_miss = 0;
   const int used = a.used[0];
   const uint32_t avail = used < 0 || used > a.pool_n ? 0u : static_cast<uint32_t>(a.pool_n - used);
-  const uint32_t rows = static_cast<uint32_t>(a.rows), page = static_cast<uint32_t>(a.page);
+  const uint32_t rows = static_cast<uint32_t>(a.rows);
   uint32_t rows_before = 0, need_before = 0;  // saturated at rows + 1 and avail + 1
   int got = 0, miss = 0;
   for (int i0 = 0; i0 < a.n; i0 += kScan * kEach) {
@@ -101,24 +117,22 @@ __global__ void __launch_bounds__(kScan) kv_extend_kernel(KvExtendArgs a) {
     int len[kEach], fresh[kEach];
     uint32_t end[kEach], upto[kEach], need[kEach], total;
     bool fits[kEach];
+    if (a.wide && i + kEach <= a.n) {
+      const int4 l = *reinterpret_cast<const int4*>(a.lens + i), f = *reinterpret_cast<const int4*>(a.fresh + i);
+      len[0] = l.x, len[1] = l.y, len[2] = l.z, len[3] = l.w;
+      fresh[0] = f.x, fresh[1] = f.y, fresh[2] = f.z, fresh[3] = f.w;
+    } else {
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      len[k] = i + k < a.n ? a.lens[i + k] : 0;
-      fresh[k] = i + k < a.n ? a.fresh[i + k] : 0;
+      for (int k = 0; k < kEach; ++k) {
+        len[k] = i + k < a.n ? a.lens[i + k] : 0;
+        fresh[k] = i + k < a.n ? a.fresh[i + k] : 0;
+      }
     }
 #pragma unroll
     for (int k = 0; k < kEach; ++k)
       end[k] = min((k ? end[k - 1] : 0u) + min(static_cast<uint32_t>(max(fresh[k], 0)), rows + 1), rows + 1);
     const uint32_t rb = rows_before;
-    uint32_t mine = end[kEach - 1];
-    uint32_t incl = block_scan(mine, rows + 1, lds, &total);
-    // (what lies before this thread: the scan without its own, which saturation forbids to subtract)
-    uint32_t prev = __shfl_up(incl, 1, 64);
-    if ((tid & 63) == 0) {
-      prev = 0;
-      for (int w = 0; w < (tid >> 6); ++w) prev = min(prev + lds[w], rows + 1);
-    }
-    prev = min(rb + prev, rows + 1);
+    uint32_t prev = min(rb + block_scan(end[kEach - 1], rows + 1, lds, &total), rows + 1);
     rows_before = min(rb + total, rows + 1);
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
@@ -127,8 +141,7 @@ __global__ void __launch_bounds__(kScan) kv_extend_kernel(KvExtendArgs a) {
                 static_cast<int64_t>(len[k]) + fresh[k] <= static_cast<int64_t>(a.width) * a.page;
       need[k] = 0;
       if (fits[k])
-        need[k] = (static_cast<uint32_t>(len[k] + fresh[k]) + page - 1) / page -
-                  (static_cast<uint32_t>(len[k]) + page - 1) / page;
+        need[k] = a.by_page.of(len[k] + fresh[k] + a.page - 1) - a.by_page.of(len[k] + a.page - 1);
       upto[k] = min((k ? upto[k - 1] : 0u) + min(need[k], avail + 1), avail + 1);
       if (i + k < a.n) {
         p.start[i + k] = static_cast<int32_t>(min(begin, rows));
@@ -136,14 +149,7 @@ __global__ void __launch_bounds__(kScan) kv_extend_kernel(KvExtendArgs a) {
       }
     }
     const uint32_t nb = need_before;
-    mine = upto[kEach - 1];
-    incl = block_scan(mine, avail + 1, lds, &total);
-    prev = __shfl_up(incl, 1, 64);
-    if ((tid & 63) == 0) {
-      prev = 0;
-      for (int w = 0; w < (tid >> 6); ++w) prev = min(prev + lds[w], avail + 1);
-    }
-    prev = min(nb + prev, avail + 1);
+    prev = min(nb + block_scan(upto[kEach - 1], avail + 1, lds, &total), avail + 1);
     need_before = min(nb + total, avail + 1);
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
@@ -171,30 +177,34 @@ __global__ void __launch_bounds__(kScan) kv_extend_kernel(KvExtendArgs a) {
     a.missed[0] = s_miss;
   }
   if constexpr (FUSED)
-    for (int r = tid; r < a.rows; r += kScan) extend_row(a, p, r);
+    for (int r = tid; r < a.rows; r += 4 * kScan) extend_rows<4>(a, p, r, kScan);
 }
 
 __global__ void __launch_bounds__(256) kv_extend_rows_kernel(KvExtendArgs a) {
-  const int r = blockIdx.x * 256 + threadIdx.x;
-  if (r < a.rows) extend_row(a, KvPlan{a.start, a.base, a.first}, r);
+  extend_rows<1>(a, KvPlan{a.start, a.base, a.first}, blockIdx.x * 256 + threadIdx.x, 0);
 }
 
 // ------------------------------------------------------------------- write
+// A copy, bound by HBM.  A workgroup takes a.chunk rows, a thread every 256th
+// of their pieces (16 bytes where all addresses allow it).  Stores that are not
+// kept in the caches leave them to the loads: 65,536 rows of 8 x 128 bf16 97
+// against 105 us, 5.5 TB/s.
 template <typename U>
 __global__ void __launch_bounds__(256) kv_write_kernel(KvWriteArgs a) {
-  const int per = a.row_bytes / static_cast<int>(sizeof(U));  // units of a head's row
-  const int64_t all = a.rows * a.heads * per;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
-    const int64_t r = i / (a.heads * per);
-    const int x = static_cast<int>(i - r * (a.heads * per));
-    const int h = x / per, u = x - h * per;
-    const int64_t slot = a.slots[r];
+  const int64_t r0 = blockIdx.x * static_cast<int64_t>(a.chunk);
+  const int rows = static_cast<int>(min(static_cast<int64_t>(a.chunk), a.rows - r0));
+  const int per = static_cast<int>(a.by_unit.d), row = per * a.heads;  // pieces of a head's row, of a row
+  for (int x = threadIdx.x; x < rows * row; x += 256) {
+    const int hr = a.by_unit.of(x), u = x - hr * per;
+    const int ri = a.by_heads.of(hr), h = hr - ri * a.heads;
+    const int64_t r = r0 + ri, slot = a.slots[r];
     if (slot < 0 || slot >= a.pages * a.page) continue;
-    const int64_t pg = slot / a.page, off = slot - pg * a.page;
-    *(reinterpret_cast<U*>(a.kc + pg * a.kc_page + h * a.kc_head + off * a.kc_tok) + u) =
-        *(reinterpret_cast<const U*>(a.k + r * a.k_row + h * a.k_head) + u);
-    *(reinterpret_cast<U*>(a.vc + pg * a.vc_page + h * a.vc_head + off * a.vc_tok) + u) =
-        *(reinterpret_cast<const U*>(a.v + r * a.v_row + h * a.v_head) + u);
+    const int pg = a.by_page.of(static_cast<int>(slot));  // (pages x page < 2^31)
+    const int64_t off = slot - static_cast<int64_t>(pg) * a.page;
+    const U k = *(reinterpret_cast<const U*>(a.k + r * a.k_row + h * a.k_head) + u);
+    const U v = *(reinterpret_cast<const U*>(a.v + r * a.v_row + h * a.v_head) + u);
+    __builtin_nontemporal_store(k, reinterpret_cast<U*>(a.kc + pg * a.kc_page + h * a.kc_head + off * a.kc_tok) + u);
+    __builtin_nontemporal_store(v, reinterpret_cast<U*>(a.vc + pg * a.vc_page + h * a.vc_head + off * a.vc_tok) + u);
   }
 }
 
@@ -205,82 +215,91 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvWriteArgs a) {
 // (a table column, or 16 bytes of a token's row of one layer) of ALL the
 // request's beams: it loads every moved beam's source before it stores, so
 // the beams may change places in any way, in place, without a second buffer.
+// A copy, bound by HBM: the workgroups that run at a time belong to few requests
+// and sweep their pages in one direction (requests in turn instead: 72 against
+// 67 us for 64 x 8 beams), stores past the caches (64 us).
 template <typename U, int JM>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorderArgs a) {
-  const int b = blockIdx.x, J = a.beams, tid = threadIdx.x;
+  const int b = blockIdx.y, J = a.beams, tid = threadIdx.x;
   __shared__ int s_par[JM], s_len[JM], s_tail[JM];
   const int64_t n0 = static_cast<int64_t>(b) * J;
   if (tid < J) {
     const int64_t p = a.parent[n0 + tid];
     const int len = a.lens[n0 + tid];
-    const int full = len < 0 ? -1 : len / a.page;
-    const bool part = len > 0 && len % a.page != 0;
+    const int full = len < 0 ? 0 : a.by_page.of(len), rest = len < 0 ? 0 : len - full * a.page;
     s_par[tid] = p >= 0 && p < J ? static_cast<int>(p) : -1;
-    s_len[tid] = len >= 0 && full + (part ? 1 : 0) <= a.width ? len : -1;
-    s_tail[tid] = part && full < a.width ? a.table[(n0 + tid) * a.table_ld + full] : -1;
+    s_len[tid] = len >= 0 && full + (rest ? 1 : 0) <= a.width ? len : -1;
+    s_tail[tid] = rest && full < a.width ? a.table[(n0 + tid) * a.table_ld + full] : -1;
   }
   __syncthreads();
   if (tid < J) {
     // beams that cannot move as asked stay as they are
     const int p = s_par[tid], len = s_len[tid];
     bool ok = p >= 0 && p != tid && len > 0 && s_len[p] == len;
-    if (ok && len % a.page != 0)
+    if (ok && len - a.by_page.of(len) * a.page != 0)
       ok = s_tail[tid] >= 0 && s_tail[tid] < a.pages && s_tail[p] >= 0 && s_tail[p] < a.pages;
     if (!ok) s_par[tid] = -1;  // (each thread reads other beams' s_len and s_tail only)
   }
   __syncthreads();
-  const int64_t step = static_cast<int64_t>(gridDim.y) * 256;
-  const int64_t me = blockIdx.y * 256ll + tid;
-  for (int64_t c = me; c < a.width; c += step) {
+  int par[JM], rest[JM];  // (the same in all threads)
+  int most = 0;
+#pragma unroll
+  for (int j = 0; j < JM; ++j) {
+    par[j] = j < J ? s_par[j] : -1;
+    rest[j] = 0;
+    if (par[j] >= 0) {
+      const int full = a.by_page.of(s_len[j]);
+      rest[j] = s_len[j] - full * a.page;
+    }
+    most = max(most, rest[j]);
+  }
+  for (int c = blockIdx.x * 256 + tid; c < a.width; c += gridDim.x * 256) {
     int32_t v[JM];
 #pragma unroll
     for (int j = 0; j < JM; ++j)
-      if (j < J && s_par[j] >= 0 && c < s_len[j] / a.page) v[j] = a.table[(n0 + s_par[j]) * a.table_ld + c];
+      if (par[j] >= 0 && c < a.by_page.of(s_len[j])) v[j] = a.table[(n0 + par[j]) * a.table_ld + c];
 #pragma unroll
     for (int j = 0; j < JM; ++j)
-      if (j < J && s_par[j] >= 0 && c < s_len[j] / a.page) a.table[(n0 + j) * a.table_ld + c] = v[j];
+      if (par[j] >= 0 && c < a.by_page.of(s_len[j])) a.table[(n0 + j) * a.table_ld + c] = v[j];
   }
-  int most = 0;
-  for (int j = 0; j < J; ++j)
-    if (s_par[j] >= 0) most = max(most, s_len[j] % a.page);
   if (most == 0) return;
-  const int per = a.row_bytes / static_cast<int>(sizeof(U));
-  const int64_t all = 2ll * a.layers * a.heads * most * per;
-  for (int64_t i = me; i < all; i += step) {
-    int64_t x = i;
-    const int u = static_cast<int>(x % per);
-    x /= per;
-    const int t = static_cast<int>(x % most);
-    x /= most;
-    const int h = static_cast<int>(x % a.heads);
-    x /= a.heads;
-    unsigned char* plane = a.kv + (x >> 1) * a.s_layer + (x & 1) * a.s_kv + h * a.s_head + t * a.s_tok;
+  // every (layer, k or v, head) plane's part-filled page, piece after piece
+  const int d = most * static_cast<int>(a.by_unit.d);
+  const FastDiv by_plane = {static_cast<uint32_t>(d), 0xffffffffu / static_cast<uint32_t>(d) + 1};
+  const int64_t all = 2ll * a.layers * a.heads * d;  // (below 2^31)
+  for (int64_t x = blockIdx.x * 256ll + tid; x < all; x += gridDim.x * 256ll) {
+    const int pl = by_plane.of(static_cast<int>(x)), i = static_cast<int>(x) - pl * d;
+    const int t = a.by_unit.of(i), u = i - t * static_cast<int>(a.by_unit.d);
+    const int lk = a.by_heads.of(pl), h = pl - lk * a.heads;
+    unsigned char* at = a.kv + (lk >> 1) * a.s_layer + (lk & 1) * a.s_kv + h * a.s_head + t * a.s_tok;
     U v[JM];
 #pragma unroll
     for (int j = 0; j < JM; ++j)
-      if (j < J && s_par[j] >= 0 && t < s_len[j] % a.page)
-        v[j] = *(reinterpret_cast<const U*>(plane + s_tail[s_par[j]] * a.s_page) + u);
+      if (t < rest[j]) v[j] = *(reinterpret_cast<const U*>(at + s_tail[par[j]] * a.s_page) + u);
 #pragma unroll
     for (int j = 0; j < JM; ++j)
-      if (j < J && s_par[j] >= 0 && t < s_len[j] % a.page)
-        *(reinterpret_cast<U*>(plane + s_tail[j] * a.s_page) + u) = v[j];
+      if (t < rest[j]) __builtin_nontemporal_store(v[j], reinterpret_cast<U*>(at + s_tail[j] * a.s_page) + u);
   }
 }
 
 template <typename U>
-void reorder_unit(const BeamReorderArgs& a, hipStream_t stream) {
-  const int64_t units = 2ll * a.layers * a.heads * a.page * (a.row_bytes / static_cast<int>(sizeof(U)));
-  int64_t gy = (units / 2 + 255) / 256;
-  gy = gy < 1 ? 1 : gy > 1024 ? 1024 : gy;
-  const dim3 grid(static_cast<uint32_t>(a.requests), static_cast<uint32_t>(gy));
-  if (a.beams <= 8) COMMEFF_LAUNCH((beam_reorder_kernel<U, 8>), grid, dim3(256), 0, stream, a);
+void reorder_unit(const BeamReorderArgs& a, int gy, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(gy), static_cast<uint32_t>(a.requests));
+  if (a.beams <= 4) COMMEFF_LAUNCH((beam_reorder_kernel<U, 4>), grid, dim3(256), 0, stream, a);
+  else if (a.beams <= 8) COMMEFF_LAUNCH((beam_reorder_kernel<U, 8>), grid, dim3(256), 0, stream, a);
   else COMMEFF_LAUNCH((beam_reorder_kernel<U, kReorderMaxBeams>), grid, dim3(256), 0, stream, a);
 }
 
 }  // namespace
 
-void launch_kv_extend(const KvExtendArgs& a, hipStream_t stream) {
-  if (a.n <= kFused && a.rows <= kFused) {
+bool kv_extend_fused(const KvExtendArgs& a) { return a.n <= kFused && a.rows <= kFused; }
+
+void launch_kv_extend(KvExtendArgs a, hipStream_t stream) {
+  a.by_page = fast_div(a.page);
+  a.search = 1;
+  while (2ll * a.search <= a.n) a.search *= 2;
+  a.wide = ((reinterpret_cast<uintptr_t>(a.lens) | reinterpret_cast<uintptr_t>(a.fresh)) & 15) == 0;
+  if (kv_extend_fused(a)) {
     const uint32_t lds = static_cast<uint32_t>(3 * a.n + 1) * 4;
     if (lds > 48 * 1024) {
       static bool attr = false;
@@ -298,22 +317,30 @@ void launch_kv_extend(const KvExtendArgs& a, hipStream_t stream) {
     COMMEFF_LAUNCH(kv_extend_rows_kernel, dim3(static_cast<uint32_t>((a.rows + 255) / 256)), dim3(256), 0, stream, a);
 }
 
-void launch_kv_write(const KvWriteArgs& a, hipStream_t stream) {
+void launch_kv_write(KvWriteArgs a, hipStream_t stream) {
   if (a.rows == 0) return;
-  const int64_t all = a.rows * a.heads * (a.row_bytes / a.unit);
-  int64_t blocks = (all + 255) / 256;
-  if (blocks > 65536) blocks = 65536;
-  const dim3 grid(static_cast<uint32_t>(blocks));
+  const int row = a.heads * (a.row_bytes / a.unit);
+  a.by_unit = fast_div(a.row_bytes / a.unit);
+  a.by_heads = fast_div(a.heads);
+  a.by_page = fast_div(a.page);
+  a.chunk = row >= 512 ? 1 : 512 / row;  // two pieces a thread, or one row
+  const dim3 grid(static_cast<uint32_t>((a.rows + a.chunk - 1) / a.chunk));
   if (a.unit == 16) COMMEFF_LAUNCH(kv_write_kernel<v4u>, grid, dim3(256), 0, stream, a);
   else if (a.unit == 4) COMMEFF_LAUNCH(kv_write_kernel<uint32_t>, grid, dim3(256), 0, stream, a);
   else COMMEFF_LAUNCH(kv_write_kernel<uint16_t>, grid, dim3(256), 0, stream, a);
 }
 
-void launch_beam_reorder(const BeamReorderArgs& a, hipStream_t stream) {
+void launch_beam_reorder(BeamReorderArgs a, hipStream_t stream) {
   if (a.requests == 0 || a.beams < 2) return;  // (one beam: its own parent)
-  if (a.unit == 16) reorder_unit<v4u>(a, stream);
-  else if (a.unit == 4) reorder_unit<uint32_t>(a, stream);
-  else reorder_unit<uint16_t>(a, stream);
+  a.by_page = fast_div(a.page);
+  a.by_heads = fast_div(a.heads);
+  a.by_unit = fast_div(a.row_bytes / a.unit);
+  // two pieces a thread where the pages are all but full
+  int64_t gy = (2ll * a.layers * a.heads * a.page * (a.row_bytes / a.unit) + 511) / 512;
+  gy = gy < 1 ? 1 : gy > 1024 ? 1024 : gy;
+  if (a.unit == 16) reorder_unit<v4u>(a, static_cast<int>(gy), stream);
+  else if (a.unit == 4) reorder_unit<uint32_t>(a, static_cast<int>(gy), stream);
+  else reorder_unit<uint16_t>(a, static_cast<int>(gy), stream);
 }
 
 }  // namespace commeff
