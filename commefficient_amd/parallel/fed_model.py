@@ -262,6 +262,16 @@ class FedModel:
     def save_pretrained(self, log_dir):
         self.model.save_pretrained(log_dir)
 
+    def generate(self, prompts, **kw):
+        """``models.gpt2.generate`` with the server weights (the bf16 replica where
+        there is one)."""
+        from ..models.gpt2 import generate
+        model = self.model
+        if self._shadow is not None:
+            self.flat.refresh_shadow()
+            model = self._shadow
+        return generate(model, prompts, **kw)
+
     def zero_grad(self):
         self.flat.zero_grad()
 

@@ -4,7 +4,8 @@ Double-heads GPT-2 (LM + multiple choice) on PersonaChat, one client per
 personality, linear LR decay from ``lr_scale`` (default 4e-2) to 0, per-round
 logging, HF ``save_pretrained`` of the server weights after each epoch,
 validation reporting nll / acc / ppl = exp(mean nll) (gpt2_train.py:149-253).
-``--finetune`` only evaluates a saved model (gpt2_train.py:308-309).
+``--finetune`` only evaluates a saved model (gpt2_train.py:308-309);
+``--replies N`` prints the model's own replies to N validation dialogues.
 With ``--synthetic`` PersonaChat-shaped token data is generated (no tokenizer
 or downloads needed); otherwise the reference on-disk layout is read with a
 local HF tokenizer directory given by ``--model_checkpoint``.
@@ -113,6 +114,38 @@ def run_batches(model, opt, sched, loader, training, args, writer=None, log_step
     return torch.cat(losses).mean().item(), torch.cat(accs).mean().item()
 
 
+def sample_replies(model, loader, args, tokenizer=None):
+    """The model's replies to the first ``args.replies`` validation dialogues that
+    leave room for one: a dict each of the dialogue, the gold reply and the reply
+    with its score (text with a tokenizer, else token ids)."""
+    special = (tokenizer.convert_tokens_to_ids(SPECIAL_TOKENS) if tokenizer is not None else
+               [args.len_tokenizer - len(SPECIAL_TOKENS) + i for i in range(len(SPECIAL_TOKENS))])
+    eos = special[1]
+    room = model.model.model.config.n_positions - args.max_reply
+    prompts, types, gold, reply_type = [], [], [], []
+    for batch in loader:
+        ids, _, lab, tt, _ = (t.cpu() for t in batch.take(np.arange(len(batch))))
+        for i, t, y in zip(ids[:, -1].tolist(), tt[:, -1].tolist(), lab[:, -1].tolist()):
+            # the gold reply is the last candidate's labelled end, behind its speaker token
+            at = next((k for k, v in enumerate(y) if v != -100), 0)
+            if len(prompts) < args.replies and 0 < at <= room:
+                prompts.append(i[:at])
+                types.append(t[:at])
+                gold.append([v for v in y[at:] if v not in (-100, eos)])
+                reply_type.append(t[at])
+        if len(prompts) >= args.replies:
+            break
+    out = [None] * len(prompts)
+    for rt in sorted(set(reply_type)):  # (one speaker, as the records are built)
+        rows = [i for i, r in enumerate(reply_type) if r == rt]
+        got = model.generate([prompts[i] for i in rows], token_types=[types[i] for i in rows], reply_type=rt,
+                             eos=eos, num_beams=args.num_beams, max_new_tokens=args.max_reply)
+        for i, (tokens, score) in zip(rows, got):
+            text = tokenizer.decode if tokenizer is not None else list
+            out[i] = {"dialogue": text(prompts[i]), "gold": text(gold[i]), "reply": text(tokens), "score": score}
+    return out
+
+
 def main(args):
     ctx = dist.init(args.device, port=args.port)
     timer = Timer()
@@ -134,6 +167,8 @@ def main(args):
     # OpenAI-GPT, gpt2_train.py:262-267 -- not the checkpoint itself)
     family = "gpt2" if "gpt2" in args.model_checkpoint else "openai-gpt"
     model = GPT2DoubleHeads(args.model_checkpoint if not args.do_test else family, **dims)
+    if args.replies and getattr(model.model.config, "model_type", "") != "gpt2":
+        raise ValueError("--replies covers GPT-2 models")
     if tokenizer is not None:
         model.model.resize_token_embeddings(len(tokenizer))
     args.len_tokenizer = model.model.config.vocab_size
@@ -165,6 +200,9 @@ def main(args):
         nll, acc = run_batches(fed, None, None, test_loader, False, args)
         if ctx.is_main:
             print({"nll": nll, "acc": acc, "ppl": math.exp(nll)})
+            if args.replies:
+                for r in sample_replies(fed, test_loader, args, tokenizer):
+                    print(r)
         return fed
     for epoch in range(progress["epoch"], math.ceil(args.num_epochs)):
         if epoch != progress["epoch"]:
@@ -192,6 +230,9 @@ def main(args):
             progress["epoch"], progress["iter"] = epoch + 1, 0
         if args.max_rounds and fed.round_idx >= args.max_rounds:
             break
+    if args.replies and ctx.is_main:
+        for r in sample_replies(fed, test_loader, args, tokenizer):
+            print(r)
     profiler.close(fed.timer)
     train_loader.close()  # the record worker processes, if any
     fed.finalize()

@@ -244,6 +244,12 @@ def build_parser(default_lr: Optional[float] = None) -> argparse.ArgumentParser:
     g.add_argument("--gpt2_size", choices=["small", "mini", "tiny"], default="small",
                    help="GPT-2 architecture: 'small' = 124M GPT-2 (reference); 'mini' (2 x 256, "
                         "4 heads: native kernels) and 'tiny' (2 x 64) for tests")
+    g.add_argument("--replies", type=int, default=0,
+                   help="GPT-2: after the evaluation of --finetune or of the last epoch, print "
+                        "the replies that the model gives to this many validation dialogues "
+                        "(beam search over a paged key-value cache, models/gpt2.py generate)")
+    g.add_argument("--num_beams", type=int, default=4, help="beams of --replies")
+    g.add_argument("--max_reply", type=int, default=20, help="longest reply of --replies, in tokens")
     return p
 
 

@@ -774,3 +774,43 @@ def test_generate_refusals():
     o = build_double_heads("openai-gpt", n_special=0, n_layer=1, n_embd=32, n_head=2)
     with pytest.raises(ValueError, match="GPT-2"):
         generate(o, [[1]])
+
+
+# ------------------------------------------------------------------- driver
+def _driver_args(tmp_path, monkeypatch, extra):
+    from commefficient_amd.utils.args import parse_args
+    monkeypatch.chdir(tmp_path)
+    return parse_args(default_lr=4e-2, argv=[
+        "--dataset_name", "PERSONA", "--synthetic", "--num_clients", "6", "--num_workers", "2",
+        "--local_batch_size", "2", "--mode", "uncompressed", "--local_momentum", "0", "--num_epochs", "1",
+        "--max_rounds", "1", "--valid_batch_size", "2", "--num_candidates", "2", "--replies", "3",
+        "--max_reply", "6", "--num_beams", "3"] + extra, probe_port=False)
+
+
+def _check_replies(printed, n_tokens):
+    rows = [eval(x, {"__builtins__": {}}, {"nan": NAN}) for x in printed.splitlines() if x.startswith("{'dialogue'")]
+    assert len(rows) == 3
+    for r in rows:
+        assert len(r["dialogue"]) > 10 and len(r["gold"]) >= 8 and len(r["reply"]) <= 6
+        assert all(0 <= t < n_tokens for t in r["reply"]) and r["score"] < 0
+
+
+def test_driver_prints_replies(tmp_path, monkeypatch, capsys):
+    from commefficient_amd.train import gpt2 as driver
+    driver.main(_driver_args(tmp_path, monkeypatch, ["--gpt2_size", "tiny", "--device", "cpu"]))
+    _check_replies(capsys.readouterr().out, 50262)
+
+
+def test_driver_refuses_replies_of_openai_gpt(tmp_path, monkeypatch):
+    from commefficient_amd.train import gpt2 as driver
+    with pytest.raises(ValueError, match="--replies"):
+        driver.main(_driver_args(tmp_path, monkeypatch, ["--gpt2_size", "tiny", "--device", "cpu",
+                                                         "--model_checkpoint", "openai-gpt"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [[], ["--finetune"]])
+def test_driver_prints_replies_native_gpu(extra, tmp_path, monkeypatch, capsys):
+    from commefficient_amd.train import gpt2 as driver
+    driver.main(_driver_args(tmp_path, monkeypatch, ["--gpt2_size", "mini", "--device", "cuda"] + extra))
+    _check_replies(capsys.readouterr().out, 50262)
