@@ -81,7 +81,7 @@ struct Elem<kF32> {
 // 64 x 12 heads of 64 bf16, up to 1,024 tokens, 27.3 against 29.6 us.
 constexpr int min_waves(int type, int dim) {
   const int row = dim * (type == kF32 ? 4 : 2);
-  return row <= 128 ? 4 : row <= 256 ? 3 : 1;
+  return row <= 128 ? 4 : row <= 256 ? 3 : 2;
 }
 
 // what a lane holds of 32 tokens: dwords of K rows and of V columns
@@ -91,8 +91,12 @@ struct Tile {
   static constexpr int KL = HD * E / 64;           // 16-byte pieces a K row leaves to a lane
   static constexpr int NC = HD / 16;               // V columns a lane holds
   static constexpr int CH = NC * E > 16 ? 16 / E : NC;  // .. of them in one load
-  v4u k[2][KL];
-  uint32_t v[8][NC * E / 4];
+  // Rows of more than 256 bytes do not fit the registers of two waves a SIMD
+  // at once: V comes in NP parts of columns, each on its way under the product
+  // of the last, K of the widest a key set at a time, and Q waits in LDS.
+  static constexpr int NP = HD * E > 256 ? HD * E / 256 : 1, NV = NC / NP;
+  v4u k[NP > 2 ? 1 : 2][KL];
+  uint32_t v[NP > 1 ? 2 : 1][8][NV * E / 4];
 };
 // column j of lane row m (of 16)
 template <DecodeType T, int HD>
@@ -106,18 +110,18 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
   typedef Elem<T> E;
   typedef typename E::t S;
   typedef Tile<T, HD> Regs;
-  constexpr int NC = Regs::NC, KL = Regs::KL, CH = Regs::CH, EB = Regs::E;
-  extern __shared__ __attribute__((aligned(16))) float lds[];  // W x min(group, 16) x (HD + 2)
+  constexpr int NC = Regs::NC, KL = Regs::KL, CH = Regs::CH, EB = Regs::E, NP = Regs::NP, NV = Regs::NV;
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // (NP > 1: Q) | W x min(group, 16) x (HD + 2)
 
-  // neighbours in the batch (the beams of a request, which share pages) on one XCD
+  // On one XCD, at about the same time: the parts of a group of more than 16
+  // heads, which read the same rows (16 x 8 heads, groups of 20, 4,096 tokens
+  // 33.9 against 37.5 us), and neighbours in the batch (the beams of a request share pages).
   int id = xcd_remap(blockIdx.x, gridDim.x);
-  int q0 = a.by_n.of(id);
-  const int n = id - q0 * a.n;
-  id = q0;
-  q0 = a.by_kv.of(id);
-  const int kh = id - q0 * a.kv_heads;
-  id = q0;
-  const int sp = a.by_tiles.of(id), gt = id - sp * static_cast<int>(a.by_tiles.d);
+  int rest = a.by_tiles.of(id);
+  const int gt = id - rest * static_cast<int>(a.by_tiles.d);
+  id = rest;
+  rest = a.by_n.of(id);
+  const int n = id - rest * a.n, sp = a.by_kv.of(rest), kh = rest - sp * a.kv_heads;
   const int cols = min(16, a.group - 16 * gt);  // query heads of this workgroup
   const int h0 = kh * a.group + 16 * gt;
 
@@ -153,10 +157,10 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
   auto look = [&](int tile) {  // the page of token lane % 32 of a tile
     return sound(row[a.by_page.of(min(tile * kTile + (lane & 31), last))]);
   };
-  auto load = [&](int tile, int ids, Regs& r) {
+  const S *kr[2], *vr[8];  // the lane's K and V rows of a tile
+  auto point = [&](int tile, int ids) {
     const int base = tile * kTile;
     const bool fresh = kn && base + kTile > last;  // the tile with the new token
-    const S *kr[2], *vr[8];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int at = min(8 * (m16 >> 2) + 4 * s + (m16 & 3), last - base), tok = base + at;
@@ -182,17 +186,18 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
       for (int i = 0; i < 8; ++i)
         if (base + 8 * g + i == last) vr[i] = vn;
     }
+  };
+  auto load_k = [&](v4u(&k)[KL], int s) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < KL; ++i)
-        r.k[s][i] = *reinterpret_cast<const v4u*>(kr[s] + i * (64 / EB) + g * (16 / EB));
+    for (int i = 0; i < KL; ++i) k[i] = *reinterpret_cast<const v4u*>(kr[s] + i * (64 / EB) + g * (16 / EB));
+  };
+  auto load_v = [&](uint32_t(&v)[8][NV * EB / 4], int part) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
-      for (int c = 0; c < NC / CH; ++c) {
-        const S* src = vr[i] + v_col<T, HD>(m16, c * CH);
-        uint32_t* dst = &r.v[i][c * CH * EB / 4];
+      for (int c = 0; c < NV / CH; ++c) {
+        const S* src = vr[i] + v_col<T, HD>(m16, part * NV + c * CH);
+        uint32_t* dst = &v[i][c * CH * EB / 4];
         if constexpr (CH * EB == 16) {
           const v4u u = *reinterpret_cast<const v4u*>(src);
           dst[0] = u[0], dst[1] = u[1], dst[2] = u[2], dst[3] = u[3];
@@ -207,13 +212,19 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
   };
 
   // Q^T: lane l holds head l % 16, the columns that it holds of a K row
-  v4u q[KL];
+  v4u* const lq = reinterpret_cast<v4u*>(lds);  // [KL][64], where it does not stay in registers
+  v4u q[NP > 1 ? 1 : KL];
+  auto q_of = [&](int i) {
+    if (m16 >= cols) return v4u{0u, 0u, 0u, 0u};
+    return *reinterpret_cast<const v4u*>(static_cast<const S*>(a.q) + n * a.q_row + (h0 + m16) * a.q_head +
+                                         i * (64 / EB) + g * (16 / EB));
+  };
+  if constexpr (NP > 1) {
+    for (int i = w; i < KL; i += W) lq[i * 64 + lane] = q_of(i);
+    __syncthreads();
+  } else {
 #pragma unroll
-  for (int i = 0; i < KL; ++i) {
-    q[i] = v4u{0u, 0u, 0u, 0u};
-    if (m16 < cols)
-      q[i] = *reinterpret_cast<const v4u*>(static_cast<const S*>(a.q) + n * a.q_row + (h0 + m16) * a.q_head +
-                                           i * (64 / EB) + g * (16 / EB));
+    for (int i = 0; i < KL; ++i) q[i] = q_of(i);
   }
   const float scale = a.scale * 1.44269504088896340736f;  // scores in powers of two
   float top = -FLT_MAX, sum = 0.f;                        // of head l % 16; sum: this lane's tokens
@@ -221,32 +232,39 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
 #pragma unroll
   for (int j = 0; j < NC; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  auto compute = [&](int tile, Regs& r) {
-    const int first = tile * kTile + 8 * g;
-    if (tile * kTile + kTile > len) {
+  auto scores = [&](const v4u(&k)[KL]) {
+    f32x4_t c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (first + i >= len) {
+    for (int i = 0; i < KL; ++i) {
+      v4u qi;
+      if constexpr (NP > 1) qi = lq[i * 64 + lane];
+      else qi = q[i];
+      if constexpr (T == kF32) {
 #pragma unroll
-          for (int c = 0; c < NC * EB / 4; ++c) r.v[i][c] = 0u;
-        }
-    }
-    f32x4_t s4[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      s4[s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        if constexpr (T == kF32) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s4[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(r.k[s][i][e]), __uint_as_float(q[i][e]),
-                                                         s4[s], 0, 0, 0);
-        } else {
-          s4[s] = E::mfma(r.k[s][i], q[i], s4[s]);
-        }
+        for (int e = 0; e < 4; ++e)
+          c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i][e]), __uint_as_float(qi[e]), c, 0, 0, 0);
+      } else {
+        c = E::mfma(k[i], qi, c);
       }
     }
+    return c;
+  };
+  auto compute = [&](int tile, int& ids, int next) {
+    Regs r;
+    const int first = tile * kTile + 8 * g;
+    f32x4_t s4[2];
+    load_k(r.k[0], 0);
+    if constexpr (NP <= 2) load_k(r.k[1], 1);
+    load_v(r.v[0], 0);
+    if (next >= 0) ids = look(next);  // (under this tile's loads)
+    s4[0] = scores(r.k[0]);
+    if constexpr (NP > 2) {
+      load_k(r.k[0], 1);
+      s4[1] = scores(r.k[0]);
+    } else {
+      s4[1] = scores(r.k[1]);
+    }
+    if constexpr (NP > 1) load_v(r.v[1], 1);
     float x[8], most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -269,29 +287,43 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
       p[i] = exp2f(x[i] - top + E::kLift);
       sum += p[i];
     }
-    if constexpr (T == kF32) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < NC; ++j)
-          o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(r.v[i][j]), p[i], o[j], 0, 0, 0);
-    } else {
-      v4u hi, lo;
+    v4u hi, lo;
+    if constexpr (T != kF32) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t u0 = E::store(p[2 * i]), u1 = E::store(p[2 * i + 1]);
         hi[i] = u0 | u1 << 16;
         lo[i] = E::store(p[2 * i] - E::load(u0)) | static_cast<uint32_t>(E::store(p[2 * i + 1] - E::load(u1))) << 16;
       }
+    }
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        v4u vt;  // row j of V^T: the lane's eight tokens
+    for (int part = 0; part < NP; ++part) {
+      auto& v = r.v[part & (NP > 1 ? 1 : 0)];
+      if (tile * kTile + kTile > len) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          vt[i] = __builtin_amdgcn_perm(r.v[2 * i + 1][j >> 1], r.v[2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
-        o[j] = E::mfma(vt, hi, o[j]);
-        o[j] = E::mfma(vt, lo, o[j]);
+        for (int i = 0; i < 8; ++i)
+          if (first + i >= len) {
+#pragma unroll
+            for (int c = 0; c < NV * EB / 4; ++c) v[i][c] = 0u;
+          }
       }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        f32x4_t& oj = o[part * NV + j];
+        if constexpr (T == kF32) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            oj = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[i][j]), p[i], oj, 0, 0, 0);
+        } else {
+          v4u vt;  // row j of V^T: the lane's eight tokens
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            vt[i] = __builtin_amdgcn_perm(v[2 * i + 1][j >> 1], v[2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+          oj = E::mfma(vt, hi, oj);
+          oj = E::mfma(vt, lo, oj);
+        }
+      }
+      if (NP > 1 && part + 2 < NP) load_v(v, part + 2);
     }
   };
 
@@ -299,10 +331,8 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
   if (t0 < t_end) {
     int ids = a.split == 1 ? sound(t0 * kTile + (lane & 31) <= last ? early : 0) : look(t0);
     for (int t = t0; t < t_end; t += W) {
-      Regs r;
-      load(t, ids, r);
-      if (t + W < t_end) ids = look(t + W);  // (under this tile's loads)
-      compute(t, r);
+      point(t, ids);
+      compute(t, ids, t + W < t_end ? t + W : -1);
     }
   }
 
@@ -321,8 +351,9 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
   sum += __shfl_xor(sum, 16, 64);
   sum += __shfl_xor(sum, 32, 64);
   if (__any(bad)) sum = NAN;
-  float* lo = lds + static_cast<size_t>(w) * cols * HD;            // [W][cols][HD]
-  float* lms = lds + static_cast<size_t>(W) * cols * HD;           // [W][cols] maxima, then sums
+  float* const lw = lds + (NP > 1 ? KL * 256 : 0);  // [W][cols][HD]
+  float* const lo = lw + w * cols * HD;
+  float* const lms = lw + W * cols * HD;            // [W][cols] maxima, then sums
   if (m16 < cols) {
     if (g == 0) {
       lms[w * cols + m16] = top;
@@ -343,7 +374,7 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const float f = exp2f(lms[i * cols + c] - mm);
-      num += f * lds[i * cols * HD + x];
+      num += f * lw[i * cols * HD + x];
       den += f * lms[(W + i) * cols + c];
     }
     const int64_t at = static_cast<int64_t>(n) * a.heads + h0 + c;
@@ -402,12 +433,13 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnArgs a) {
 template <DecodeType T, int HD, int W>
 void launch_one(const PagedAttnArgs& a, hipStream_t stream) {
   const int group = a.heads / a.kv_heads, cols = group < 16 ? group : 16;
-  const uint32_t lds = static_cast<uint32_t>(W * cols * (HD + 2) * 4);
+  typedef Tile<T, HD> Regs;
+  const uint32_t lds = static_cast<uint32_t>(W * cols * (HD + 2) * 4 + (Regs::NP > 1 ? Regs::KL * 1024 : 0));
   if (lds > 65536) {
     static bool attr = false;
     if (!attr) {
       (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, HD, W>),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+                                hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
       attr = true;
     }
   }
