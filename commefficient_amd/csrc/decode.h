@@ -108,7 +108,8 @@ struct BeamSelectArgs {
   int64_t s_request, s_beam;  // elements
   int64_t eos;
   int requests, beams, vocab, keep, parts;
-  FastDiv by_beams, by_parts, by_lists;  // launch_beam_select
+  int tight;                             // launch_beam_select
+  FastDiv by_beams, by_parts, by_lists;
 };
 
 bool kv_extend_fused(const KvExtendArgs& a);  // one launch, the plan in LDS

@@ -232,6 +232,7 @@ void check_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc,
   check_page(kc.size(2), 0, op);
   TORCH_CHECK(kc.size(0) * kc.size(2) < (1ll << 31), op, ": the caches must hold less than 2^31 slots, not ",
               kc.size(0), " pages of ", kc.size(2));
+  TORCH_CHECK(kc.numel() == 0 || kc.data_ptr() != vc.data_ptr(), op, ": key and value cache are the same");
   check_rows(k, -1, kc, op, "k");
   TORCH_CHECK(k.size(0) < (1ll << 31) && k.size(1) * k.size(2) <= (1ll << 24), op, ": rows too many or too long: ",
               k.sizes());
@@ -379,6 +380,7 @@ void check_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
   TORCH_CHECK(q.size(0) * q.size(1) <= (1ll << 24), op, ": at most 2^24 sequences x heads");
   TORCH_CHECK(given(k) == given(v), op, ": k and v come together");
   if (given(k)) {
+    TORCH_CHECK(kc.data_ptr() != vc.data_ptr(), op, ": key and value cache are the same");
     check_rows(*k, q.size(0), kc, op, "k");
     check_rows(*v, q.size(0), vc, op, "v");
   }

@@ -301,14 +301,9 @@ void launch_kv_extend(KvExtendArgs a, hipStream_t stream) {
   a.wide = ((reinterpret_cast<uintptr_t>(a.lens) | reinterpret_cast<uintptr_t>(a.fresh)) & 15) == 0;
   if (kv_extend_fused(a)) {
     const uint32_t lds = static_cast<uint32_t>(3 * a.n + 1) * 4;
-    if (lds > 48 * 1024) {
-      static bool attr = false;
-      if (!attr) {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kv_extend_kernel<true>),
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, (3 * kFused + 1) * 4);
-        attr = true;
-      }
-    }
+    if (lds > 65536 - 1024)  // (of the current device: set wherever it is needed)
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kv_extend_kernel<true>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (3 * kFused + 1) * 4);
     COMMEFF_LAUNCH(kv_extend_kernel<true>, dim3(1), dim3(kScan), lds, stream, a);
     return;
   }

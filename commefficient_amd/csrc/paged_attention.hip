@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
     if (__any(m16 < cols && most > top + E::kSlack)) {
       most = fmaxf(most, __shfl_xor(most, 16, 64));
       most = fmaxf(most, __shfl_xor(most, 32, 64));
-      const float now = fmaxf(top, most), c = exp2f(top - now);
+      const float now = fmaxf(top, most), c = __builtin_amdgcn_exp2f(top - now);
       top = now;
       sum *= c;
 #pragma unroll
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[i] = exp2f(x[i] - top + E::kLift);
+      p[i] = __builtin_amdgcn_exp2f(x[i] - top + E::kLift);
       sum += p[i];
     }
     v4u hi, lo;
@@ -435,14 +435,9 @@ void launch_one(const PagedAttnArgs& a, hipStream_t stream) {
   const int group = a.heads / a.kv_heads, cols = group < 16 ? group : 16;
   typedef Tile<T, HD> Regs;
   const uint32_t lds = static_cast<uint32_t>(W * cols * (HD + 2) * 4 + (Regs::NP > 1 ? Regs::KL * 1024 : 0));
-  if (lds > 65536) {
-    static bool attr = false;
-    if (!attr) {
-      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, HD, W>),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
-      attr = true;
-    }
-  }
+  if (lds > 65536)  // (of the current device: set wherever it is needed)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, HD, W>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
   const uint32_t blocks = static_cast<uint32_t>(a.n) * a.kv_heads * ((group + 15) / 16) * a.split;
   COMMEFF_LAUNCH((paged_attn_kernel<T, HD, W>), dim3(blocks), dim3(W * 64), lds, stream, a);
   if (a.split > 1)

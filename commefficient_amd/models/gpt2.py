@@ -160,8 +160,8 @@ def generate(model, prompts, *, max_new_tokens=20, num_beams=4, eos=None, token_
     lens = [len(p) for p in prompts]
     if not lens:
         return []
-    if min(lens) < 1 or max_new_tokens < 1 or num_beams < 1:
-        raise ValueError("generate() needs a token in every prompt, a new token and a beam")
+    if min(lens) < 1 or max_new_tokens < 1 or not 1 <= num_beams <= 32:
+        raise ValueError("generate() needs a token in every prompt, a new token and 1 to 32 beams")
     if max(lens) + max_new_tokens > cfg.n_positions:
         raise ValueError("a prompt of %d tokens and %d new ones are more than the model's %d positions"
                          % (max(lens), max_new_tokens, cfg.n_positions))

@@ -177,12 +177,14 @@ def test_write_refusals():
     ok = dict(k=z(3, 2, 4), v=z(3, 2, 4), k_cache=z(5, 2, 8, 4), v_cache=z(5, 2, 8, 4),
               slots=torch.arange(3))
     decode.kv_write(**ok)
-    for bad in (dict(k=z(3, 2, 5)), dict(v=z(2, 2, 4)), dict(k=z(3, 2, 4).to(BF)), dict(v_cache=z(5, 2, 8, 5)),
+    for bad in (dict(k=z(3, 2, 5)), dict(v=z(2, 2, 4)), dict(k=z(3, 2, 4).to(BF)), dict(v_cache=z(5, 2, 8, 5)), dict(v_cache="k_cache"),
                 dict(k_cache=z(5, 2, 4, 8).transpose(2, 3)), dict(k_cache=z(1, 2, 8, 4).expand(5, 2, 8, 4)),
                 dict(slots=torch.arange(2)), dict(slots=torch.arange(3).int()),
                 dict(k=z(3, 2, 4, requires_grad=True)),
                 dict(k=z(3, 2, 4).double(), v=z(3, 2, 4).double(), k_cache=z(5, 2, 8, 4).double(),
                      v_cache=z(5, 2, 8, 4).double())):
+        if bad.get("v_cache") == "k_cache":
+            bad = dict(v_cache=ok["k_cache"])
         with pytest.raises(RuntimeError, match="kv_write"):
             decode.kv_write(**{**ok, **bad})
 
@@ -473,13 +475,20 @@ def _select_case(name):
         return 40 * rnd(3, 5, 2049), 9 * rnd(3, 5), 10, None, -1
     if name == "sorted":  # the best all in one stretch of the row
         return (torch.arange(30000.) / 1000).expand(2, 2, 30000).contiguous(), rnd(2, 2), 64, None, -1
+    if name == "batch":  # enough rows for the bound that the waves share, in steps and in ties
+        x = rnd(40, 4, 33001)
+        x[::3] = (x[::3] * 2).round() / 2
+        x[5, 1] = -INF
+        x[5, 1, 77] = 0.0
+        x[6, :, 100:] = -INF
+        return x.to(BF), rnd(40, 4).mul(8).round() / 8 + torch.arange(4) / 3, 16, None, -1
     if name == "huge":
         return rnd(1, 2, 250007), rnd(1, 2), 4, None, -1
     raise KeyError(name)
 
 
 @pytest.mark.parametrize("name", ["one", "few", "odd", "wide", "padded", "unaligned", "columns", "first", "equal",
-                                  "steps", "masked", "dead", "finished", "spread", "sorted", "huge"])
+                                  "steps", "masked", "dead", "finished", "spread", "sorted", "batch", "huge"])
 @pytest.mark.parametrize("device", DEVICES)
 def test_select(device, name):
     """Scores are off by fp32's rounding of the result and, on the GPU, by a log of a sum
@@ -635,6 +644,18 @@ def _run_steps(s, step, steps):
     assert int(s.cache.missed) == 0
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_inference_mode_and_grad_mode(device):
+    """The operators run under inference_mode, and on tensors of it afterwards."""
+    with torch.inference_mode():
+        s = _Steps(device)
+        s.step()
+        s.step()
+        assert int(s.cache.missed) == 0 and s.cache.lens.cpu().tolist() == [2] * 12
+    r = decode.kv_extend(s.cache.table.clone(), s.cache.lens, s.one, s.cache.pool, s.cache.used, 4, 12)
+    assert r.lens.cpu().tolist() == [3] * 12 and s.cache.lens.cpu().tolist() == [2] * 12
+
+
 @pytest.mark.parametrize("page", [1, 4, 16])
 @pytest.mark.parametrize("device", DEVICES)
 def test_steps_together(device, page):
@@ -766,7 +787,7 @@ def test_generate_native_bf16_gpu():
 def test_generate_refusals():
     m = _tiny(64, 2, FP, "cpu", n_positions=32)
     assert generate(m, []) == []
-    for kw in (dict(prompts=[[1], []]), dict(prompts=[[1]], max_new_tokens=0), dict(prompts=[[1]], num_beams=0),
+    for kw in (dict(prompts=[[1], []]), dict(prompts=[[1]], max_new_tokens=0), dict(prompts=[[1]], num_beams=0), dict(prompts=[[1]], num_beams=33),
                dict(prompts=[[1] * 20], max_new_tokens=13), dict(prompts=[[1]], token_types=[[1]]),
                dict(prompts=[[1, 2]], token_types=[[1]], reply_type=1), dict(prompts=[[1]], eos=50262)):
         with pytest.raises(ValueError):
