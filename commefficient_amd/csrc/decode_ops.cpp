@@ -121,14 +121,14 @@ std::vector<at::Tensor> extend_outputs(at::Tensor& table, at::Tensor& lens, cons
   TORCH_CHECK(n <= (1ll << 30) && pool.numel() <= (1ll << 30), op, ": at most 2^30 sequences and pages");
   auto i32 = lens.options();
   // slots [rows] | one allocation: pos [rows], seq [rows], start [n + 1], missed (, lens [n], used)
-  const int64_t all = 2 * rows + n + 2 + (in_place ? 0 : n + 1);
+  const int64_t all = 2 * (rows + 3) + n + 1 + 3 + 4 + (in_place ? 0 : n + 3 + 4);
   const auto buf = at::empty({all}, i32);
   int64_t at = 0;
   auto piece = [&](int64_t size) {  // (a narrow() without the dispatcher: half of this call's host time otherwise)
     auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
     t->set_storage_offset(at);
     t->set_sizes_contiguous({size});
-    at += size;
+    at += (size + 3) / 4 * 4;  // (each at a multiple of 16 bytes)
     return at::Tensor(std::move(t));
   };
   std::vector<at::Tensor> out;

@@ -51,50 +51,76 @@ struct KvPlan {  // of the sequences: LDS, or global memory
   int32_t *start, *base, *first;
 };
 
-// rows r, r + step, ..: slot, position, sequence, and the table entry where one
-// opens a page.  ROWS searches, and then loads, of a thread run side by side.
-template <int ROWS>
-__device__ __forceinline__ void extend_rows(const KvExtendArgs& a, const KvPlan& p, int r0, int step) {
-  int seq[ROWS], pos[ROWS], off[ROWS];
-  const int32_t* src[ROWS];
-  int32_t* dst[ROWS];
+// rows r0 .. r0 + 3: slot, position, sequence, and the table entry where one
+// opens a page.  One search for the four: the later rows mostly belong to the
+// same sequence or the next (4,096 rows on one CU are bound by instructions).
+__device__ __forceinline__ void extend_rows(const KvExtendArgs& a, const KvPlan& p, int r0) {
+  if (r0 >= a.rows) return;
+  int i = 0;  // the sequences that end at or before the row: start[i] <= r for i <= that many
+  auto search = [&](int r) {
+    i = 0;
+    for (int s = a.search; s > 0; s >>= 1)
+      if (i + s <= a.n && p.start[i + s] <= r) i += s;
+  };
+  search(r0);
+  int seq[4], pos[4], off[4], id[4];
+  const int32_t* src[4];
+  int32_t* dst[4];
+  int end = i < a.n ? p.start[i + 1] : 0x7fffffff, len = -1, begin = 0, have = 0;
+  const int32_t* taken = nullptr;
+  int32_t* row = nullptr;
+  bool enter = true;
 #pragma unroll
-  for (int k = 0; k < ROWS; ++k) seq[k] = 0;
-  // the sequences that end at or before the row: start[i] <= r for i <= that many
-  for (int s = a.search; s > 0; s >>= 1)
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k)
-      if (seq[k] + s <= a.n && p.start[seq[k] + s] <= r0 + k * step) seq[k] += s;
-#pragma unroll
-  for (int k = 0; k < ROWS; ++k) {
-    const int i = seq[k], r = r0 + k * step;
-    const int len = i < a.n && r < a.rows ? p.base[i] : -1;
+  for (int k = 0; k < 4; ++k) {
+    const int r = r0 + k;
+    if (r >= end && r < a.rows) {
+      ++i;
+      end = i < a.n ? p.start[i + 1] : 0x7fffffff;
+      if (r >= end) {  // (empty sequences between)
+        search(r);
+        end = i < a.n ? p.start[i + 1] : 0x7fffffff;
+      }
+      enter = true;
+    }
+    if (enter) {
+      enter = false;
+      len = i < a.n ? p.base[i] : -1;
+      if (len >= 0) {
+        begin = p.start[i];
+        have = a.by_page.of(len + a.page - 1);
+        row = a.table + i * a.table_ld;
+        taken = a.pool + p.first[i];
+      }
+    }
+    seq[k] = i < a.n ? i : -1;
     src[k] = nullptr;
     dst[k] = nullptr;
     pos[k] = off[k] = 0;
-    if (len >= 0) {
-      pos[k] = len + r - p.start[i];
-      const int pi = a.by_page.of(pos[k]), have = a.by_page.of(len + a.page - 1);
+    if (len >= 0 && r < a.rows) {
+      pos[k] = len + r - begin;
+      const int pi = a.by_page.of(pos[k]);
       off[k] = pos[k] - pi * a.page;
-      int32_t* row = a.table + i * a.table_ld + pi;
-      src[k] = row;
-      if (pi >= have) {
-        src[k] = a.pool + p.first[i] + pi - have;
-        if (off[k] == 0) dst[k] = row;
-      }
+      src[k] = pi < have ? row + pi : taken + (pi - have);
+      if (pi >= have && off[k] == 0) dst[k] = row + pi;
     }
   }
-  int id[ROWS];
+  int64_t slot[4];
 #pragma unroll
-  for (int k = 0; k < ROWS; ++k) id[k] = src[k] ? *src[k] : -1;
+  for (int k = 0; k < 4; ++k) id[k] = src[k] ? *src[k] : -1;
 #pragma unroll
-  for (int k = 0; k < ROWS; ++k) {
-    const int r = r0 + k * step;
-    if (r >= a.rows) continue;
+  for (int k = 0; k < 4; ++k) {
     if (dst[k]) *dst[k] = id[k];
-    a.slots[r] = id[k] < 0 ? -1 : static_cast<int64_t>(id[k]) * a.page + off[k];
-    a.pos[r] = pos[k];
-    a.seq[r] = seq[k] < a.n ? seq[k] : -1;
+    slot[k] = id[k] < 0 ? -1 : static_cast<int64_t>(id[k]) * a.page + off[k];
+  }
+  if (r0 + 4 <= a.rows) {  // (the outputs start at multiples of 16 bytes)
+    *reinterpret_cast<longlong2*>(a.slots + r0) = longlong2{slot[0], slot[1]};
+    *reinterpret_cast<longlong2*>(a.slots + r0 + 2) = longlong2{slot[2], slot[3]};
+    *reinterpret_cast<int4*>(a.pos + r0) = int4{pos[0], pos[1], pos[2], pos[3]};
+    *reinterpret_cast<int4*>(a.seq + r0) = int4{seq[0], seq[1], seq[2], seq[3]};
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (r0 + k < a.rows) a.slots[r0 + k] = slot[k], a.pos[r0 + k] = pos[k], a.seq[r0 + k] = seq[k];
   }
 }
 
@@ -177,11 +203,11 @@ __global__ void __launch_bounds__(kScan) kv_extend_kernel(KvExtendArgs a) {
     a.missed[0] = s_miss;
   }
   if constexpr (FUSED)
-    for (int r = tid; r < a.rows; r += 4 * kScan) extend_rows<4>(a, p, r, kScan);
+    for (int r = tid * 4; r < a.rows; r += 4 * kScan) extend_rows(a, p, r);
 }
 
 __global__ void __launch_bounds__(256) kv_extend_rows_kernel(KvExtendArgs a) {
-  extend_rows<1>(a, KvPlan{a.start, a.base, a.first}, blockIdx.x * 256 + threadIdx.x, 0);
+  extend_rows(a, KvPlan{a.start, a.base, a.first}, (blockIdx.x * 256 + threadIdx.x) * 4);
 }
 
 // ------------------------------------------------------------------- write
@@ -309,7 +335,7 @@ void launch_kv_extend(KvExtendArgs a, hipStream_t stream) {
   }
   COMMEFF_LAUNCH(kv_extend_kernel<false>, dim3(1), dim3(kScan), 0, stream, a);
   if (a.rows > 0)
-    COMMEFF_LAUNCH(kv_extend_rows_kernel, dim3(static_cast<uint32_t>((a.rows + 255) / 256)), dim3(256), 0, stream, a);
+    COMMEFF_LAUNCH(kv_extend_rows_kernel, dim3(static_cast<uint32_t>((a.rows + 1023) / 1024)), dim3(256), 0, stream, a);
 }
 
 void launch_kv_write(KvWriteArgs a, hipStream_t stream) {
