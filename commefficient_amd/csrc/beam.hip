@@ -127,10 +127,13 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
   const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / EB;
   const int pieces = (skew + a.vocab + GE - 1) / GE;
   const int per = a.by_parts.of(pieces + a.parts - 1), end = min(pieces, (part + 1) * per);
+  // pieces by thread; where they are too few for a bound, over all waves: their
+  // lists then hold every element
+  const int mine_pc = part * per + (per < a.keep ? lane * 4 + w : tid);
   v4u u[kPieces];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    const int pc = part * per + i * kThreads + tid;
+    const int pc = mine_pc + i * kThreads;
     const int v0 = pc * GE - skew;
     u[i] = v4u{kLow<T>, kLow<T>, kLow<T>, kLow<T>};
     if (pc < end && v0 >= 0 && v0 + GE <= a.vocab) {
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
         const u64 mask = __ballot(in);
         if (mask == 0) continue;
         const int c = mine + __popcll(mask & ((1ull << lane) - 1));
-        if (in && c < kList) s_list[w][c] = key(at(i, e), (part * per + i * kThreads + tid) * GE - skew + e);
+        if (in && c < kList) s_list[w][c] = key(at(i, e), (mine_pc + i * kThreads) * GE - skew + e);
         mine += __popcll(mask);
       }
     }
@@ -226,16 +229,20 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
   __syncthreads();
   const int most_n = max(max(s_n[0], s_n[1]), max(s_n[2], s_n[3])), n = s_n[0] + s_n[1] + s_n[2] + s_n[3];
   if (most_n <= kList) {
-    // a wave ranks its own list, four lanes a candidate, each against one list
-    const int q = lane & 3, nq = s_n[q];
-    for (int c = lane >> 2; c < mine; c += 16) {
-      const u64 k = s_list[w][c];
+    // four lanes a candidate, each against every fourth one of all lists
+    for (int c = tid >> 2; c < n; c += kThreads / 4) {
+      int l = 0, i0 = c;
+      while (i0 >= s_n[l]) i0 -= s_n[l++];
+      const u64 k = s_list[l][i0];
       int rank = 0;
+      for (int q = 0; q < 4; ++q) {
+        const int nq = s_n[q];
 #pragma unroll 4
-      for (int i = 0; i < nq; ++i) rank += s_list[q][i] > k;
+        for (int i = tid & 3; i < nq; i += 4) rank += s_list[q][i] > k;
+      }
       rank += __shfl_xor(rank, 1, 64);
       rank += __shfl_xor(rank, 2, 64);
-      if (q == 0 && rank < a.keep) cand[rank] = k;
+      if ((tid & 3) == 0 && rank < a.keep) cand[rank] = k;
     }
     for (int k = n + tid; k < a.keep; k += kThreads) cand[k] = 0;
     return;
@@ -264,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   constexpr int kHeld = 4;  // candidates a thread holds
   __shared__ Best s_list[kJoinList];
   __shared__ Best s_best[4];
-  __shared__ uint32_t s_u[4];
+  __shared__ uint32_t s_u[2][4];
   __shared__ int s_n;
   extern __shared__ __attribute__((aligned(16))) double s_lse[];  // [beams], +inf: no continuation by its logits
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -327,10 +334,29 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   }
   for (int c = tid + kHeld * kThreads; c < all; c += kThreads)
     most = max(most, static_cast<uint32_t>(score(c, fetch(c)).value >> 32));
-  uint32_t bound = wave_bound(most, a.keep);
-  if (lane == 0) s_u[w] = bound;
-  __syncthreads();
-  bound = max(max(s_u[0], s_u[1]), max(max(s_u[2], s_u[3]), 1u));
+  uint32_t bound = 0;
+  if (a.keep <= 32 || all > kHeld * kThreads) {
+    bound = wave_bound(most, a.keep);
+    if (lane == 0) s_u[0][w] = bound;
+    __syncthreads();
+    bound = max(max(s_u[0][0], s_u[0][1]), max(s_u[0][2], s_u[0][3]));
+  } else {
+    // many places: the keep-th largest of all candidates, so that few more than
+    // those are left to rank (16 beams, 64 places: 13.0 against
+    // 150 us; for up to 32 the search costs what it saves)
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t c = bound | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) n += __popcll(__ballot(static_cast<uint32_t>(mine[i].value >> 32) >= c));
+      if (lane == 0) s_u[bit & 1][w] = n;
+      __syncthreads();  // (the other half is read until the next one)
+      n = s_u[bit & 1][0] + s_u[bit & 1][1] + s_u[bit & 1][2] + s_u[bit & 1][3];
+      if (n >= a.keep) bound = c;
+      if (n == a.keep) break;
+    }
+  }
+  bound = max(bound, 1u);
   auto pass = [&](const Best& x) {
     if (static_cast<uint32_t>(x.value >> 32) >= bound) {
       const int at = atomicAdd(&s_n, 1);  // (any order: the list is ranked)

@@ -247,12 +247,14 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvWriteArgs a) {
 template <typename U, int JM>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorderArgs a) {
   const int b = blockIdx.y, J = a.beams, tid = threadIdx.x;
-  __shared__ int s_par[JM], s_len[JM], s_tail[JM];
+  __shared__ int s_len[JM], s_tail[JM], s_par[JM];
+  __shared__ int s_from[JM], s_full[JM], s_rest[JM];  // the parent's part-filled page, and what to take (0: nothing)
   const int64_t n0 = static_cast<int64_t>(b) * J;
+  int len = 0, full = 0, rest = 0;
   if (tid < J) {
+    len = a.lens[n0 + tid];
+    full = len < 0 ? 0 : a.by_page.of(len), rest = len < 0 ? 0 : len - full * a.page;
     const int64_t p = a.parent[n0 + tid];
-    const int len = a.lens[n0 + tid];
-    const int full = len < 0 ? 0 : a.by_page.of(len), rest = len < 0 ? 0 : len - full * a.page;
     s_par[tid] = p >= 0 && p < J ? static_cast<int>(p) : -1;
     s_len[tid] = len >= 0 && full + (rest ? 1 : 0) <= a.width ? len : -1;
     s_tail[tid] = rest && full < a.width ? a.table[(n0 + tid) * a.table_ld + full] : -1;
@@ -260,34 +262,26 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorderArgs a) {
   __syncthreads();
   if (tid < J) {
     // beams that cannot move as asked stay as they are
-    const int p = s_par[tid], len = s_len[tid];
-    bool ok = p >= 0 && p != tid && len > 0 && s_len[p] == len;
-    if (ok && len - a.by_page.of(len) * a.page != 0)
+    const int p = s_par[tid];
+    bool ok = p >= 0 && p != tid && s_len[tid] > 0 && s_len[p] == len;
+    if (ok && rest)
       ok = s_tail[tid] >= 0 && s_tail[tid] < a.pages && s_tail[p] >= 0 && s_tail[p] < a.pages;
-    if (!ok) s_par[tid] = -1;  // (each thread reads other beams' s_len and s_tail only)
+    s_from[tid] = ok ? s_tail[p] : 0;
+    s_full[tid] = ok ? full : 0;
+    s_rest[tid] = ok ? rest : 0;
   }
   __syncthreads();
-  int par[JM], rest[JM];  // (the same in all threads)
-  int most = 0;
-#pragma unroll
-  for (int j = 0; j < JM; ++j) {
-    par[j] = j < J ? s_par[j] : -1;
-    rest[j] = 0;
-    if (par[j] >= 0) {
-      const int full = a.by_page.of(s_len[j]);
-      rest[j] = s_len[j] - full * a.page;
-    }
-    most = max(most, rest[j]);
-  }
   for (int c = blockIdx.x * 256 + tid; c < a.width; c += gridDim.x * 256) {
     int32_t v[JM];
 #pragma unroll
     for (int j = 0; j < JM; ++j)
-      if (par[j] >= 0 && c < a.by_page.of(s_len[j])) v[j] = a.table[(n0 + par[j]) * a.table_ld + c];
+      if (j < J && c < s_full[j]) v[j] = a.table[(n0 + s_par[j]) * a.table_ld + c];
 #pragma unroll
     for (int j = 0; j < JM; ++j)
-      if (par[j] >= 0 && c < a.by_page.of(s_len[j])) a.table[(n0 + j) * a.table_ld + c] = v[j];
+      if (j < J && c < s_full[j]) a.table[(n0 + j) * a.table_ld + c] = v[j];
   }
+  int most = 0;
+  for (int j = 0; j < J; ++j) most = max(most, s_rest[j]);
   if (most == 0) return;
   // every (layer, k or v, head) plane's part-filled page, piece after piece
   const int d = most * static_cast<int>(a.by_unit.d);
@@ -301,10 +295,11 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorderArgs a) {
     U v[JM];
 #pragma unroll
     for (int j = 0; j < JM; ++j)
-      if (t < rest[j]) v[j] = *(reinterpret_cast<const U*>(at + s_tail[par[j]] * a.s_page) + u);
+      if (j < J && t < s_rest[j]) v[j] = *(reinterpret_cast<const U*>(at + s_from[j] * a.s_page) + u);
 #pragma unroll
     for (int j = 0; j < JM; ++j)
-      if (t < rest[j]) __builtin_nontemporal_store(v[j], reinterpret_cast<U*>(at + s_tail[j] * a.s_page) + u);
+      if (j < J && t < s_rest[j])
+        __builtin_nontemporal_store(v[j], reinterpret_cast<U*>(at + s_tail[j] * a.s_page) + u);
   }
 }
 
@@ -313,6 +308,7 @@ void reorder_unit(const BeamReorderArgs& a, int gy, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(gy), static_cast<uint32_t>(a.requests));
   if (a.beams <= 4) COMMEFF_LAUNCH((beam_reorder_kernel<U, 4>), grid, dim3(256), 0, stream, a);
   else if (a.beams <= 8) COMMEFF_LAUNCH((beam_reorder_kernel<U, 8>), grid, dim3(256), 0, stream, a);
+  else if (a.beams <= 16) COMMEFF_LAUNCH((beam_reorder_kernel<U, 16>), grid, dim3(256), 0, stream, a);
   else COMMEFF_LAUNCH((beam_reorder_kernel<U, kReorderMaxBeams>), grid, dim3(256), 0, stream, a);
 }
 

@@ -79,9 +79,9 @@ struct Elem<kF32> {
 // Waves a SIMD holds at least, by a token's row in bytes.  Many waves with one
 // tile each in flight beat fewer that load the next tile under the products:
 // 64 x 12 heads of 64 bf16, up to 1,024 tokens, 27.3 against 29.6 us.
-constexpr int min_waves(int type, int dim) {
+constexpr int min_waves(int type, int dim, int few) {
   const int row = dim * (type == kF32 ? 4 : 2);
-  return row <= 128 ? 4 : row <= 256 ? 3 : 2;
+  return row <= (few == 1 ? 256 : 128) ? 4 : row <= 256 ? 3 : 2;
 }
 
 // what a lane holds of 32 tokens: dwords of K rows and of V columns
@@ -105,13 +105,20 @@ __device__ __forceinline__ int v_col(int m, int j) {
   return (j / CH) * (16 * CH) + m * CH + j % CH;
 }
 
-template <DecodeType T, int HD, int W>
-__global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(PagedAttnArgs a) {
+// FEW > 0 (fp32, groups of FEW = 1 or 2 heads): the products on the
+// vector units, head by head.  The fp32 MFMA works on 16 columns whatever the
+// group needs, 8,192 cycles for 32 tokens of 256 columns against 1,100 a head
+// here (4 sequences x 4 heads of 256, 600 tokens, 27.8 against 47.9 us; 33 x 12 of
+// 64, up to 777 tokens, 22.1 against 28.0).  A lane then has the scores
+// of tokens m16 of both key sets, summed over the lanes g, and its columns'
+// sums of tokens 8 g .. + 7, joined at the end.
+template <DecodeType T, int HD, int W, int FEW>
+__global__ void __launch_bounds__(W * 64, min_waves(T, HD, FEW)) paged_attn_kernel(PagedAttnArgs a) {
   typedef Elem<T> E;
   typedef typename E::t S;
   typedef Tile<T, HD> Regs;
   constexpr int NC = Regs::NC, KL = Regs::KL, CH = Regs::CH, EB = Regs::E, NP = Regs::NP, NV = Regs::NV;
-  extern __shared__ __attribute__((aligned(16))) float lds[];  // (NP > 1: Q) | W x min(group, 16) x (HD + 2)
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // (Q) | W x min(group, 16) x (HD + 2)
 
   // On one XCD, at about the same time: the parts of a group of more than 16
   // heads, which read the same rows (16 x 8 heads, groups of 20, 4,096 tokens
@@ -213,13 +220,23 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
 
   // Q^T: lane l holds head l % 16, the columns that it holds of a K row
   v4u* const lq = reinterpret_cast<v4u*>(lds);  // [KL][64], where it does not stay in registers
-  v4u q[NP > 1 ? 1 : KL];
+  v4u q[NP > 1 || FEW > 0 ? 1 : KL];
   auto q_of = [&](int i) {
     if (m16 >= cols) return v4u{0u, 0u, 0u, 0u};
     return *reinterpret_cast<const v4u*>(static_cast<const S*>(a.q) + n * a.q_row + (h0 + m16) * a.q_head +
                                          i * (64 / EB) + g * (16 / EB));
   };
-  if constexpr (NP > 1) {
+  if constexpr (FEW > 0) {  // [FEW][KL][4 lanes g]
+    for (int x = tid; x < FEW * KL * 4; x += W * 64) {
+      const int h = x / (KL * 4), i = x / 4 % KL;
+      v4u u = {0u, 0u, 0u, 0u};
+      if (h < cols)
+        u = *reinterpret_cast<const v4u*>(static_cast<const S*>(a.q) + n * a.q_row + (h0 + h) * a.q_head +
+                                          i * (64 / EB) + x % 4 * (16 / EB));
+      lq[x] = u;
+    }
+    __syncthreads();
+  } else if constexpr (NP > 1) {
     for (int i = w; i < KL; i += W) lq[i * 64 + lane] = q_of(i);
     __syncthreads();
   } else {
@@ -327,12 +344,97 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
     }
   };
 
+  // the same, head by head
+  constexpr int NF = FEW > 0 ? FEW : 1;
+  float ftop[NF], fsum[NF], fo[NF][FEW > 0 ? NC : 1];
+#pragma unroll
+  for (int h = 0; h < NF; ++h) {
+    ftop[h] = -FLT_MAX;
+    fsum[h] = 0.f;
+#pragma unroll
+    for (int j = 0; j < (FEW > 0 ? NC : 1); ++j) fo[h][j] = 0.f;
+  }
+  auto compute_few = [&](int tile, int& ids, int next) {
+    Regs r;
+    const int base = tile * kTile, first = base + 8 * g;
+    float x[NF][2];
+    load_k(r.k[0], 0);
+    if constexpr (NP <= 2) load_k(r.k[1], 1);
+    load_v(r.v[0], 0);
+    if (next >= 0) ids = look(next);
+    auto dot = [&](const v4u(&k)[KL], int s) {
+#pragma unroll
+      for (int h = 0; h < NF; ++h) {
+        float c0 = 0.f, c1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          const v4u u = lq[(h * KL + i) * 4 + g];
+          c0 = fmaf(__uint_as_float(k[i][0]), __uint_as_float(u[0]), c0);
+          c1 = fmaf(__uint_as_float(k[i][1]), __uint_as_float(u[1]), c1);
+          c0 = fmaf(__uint_as_float(k[i][2]), __uint_as_float(u[2]), c0);
+          c1 = fmaf(__uint_as_float(k[i][3]), __uint_as_float(u[3]), c1);
+        }
+        c0 += c1;
+        c0 += __shfl_xor(c0, 16, 64);
+        c0 += __shfl_xor(c0, 32, 64);
+        x[h][s] = base + 8 * (m16 >> 2) + 4 * s + (m16 & 3) < len ? c0 * scale : -INFINITY;
+      }
+    };
+    dot(r.k[0], 0);
+    if constexpr (NP > 2) {
+      load_k(r.k[0], 1);
+      dot(r.k[0], 1);
+    } else {
+      dot(r.k[1], 1);
+    }
+    if constexpr (NP > 1) load_v(r.v[1], 1);
+    float p[NF][8];
+#pragma unroll
+    for (int h = 0; h < NF; ++h) {
+      float most = fmaxf(x[h][0], x[h][1]);
+      if (__any(most > ftop[h] + E::kSlack)) {
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+        const float now = fmaxf(ftop[h], most), c = __builtin_amdgcn_exp2f(ftop[h] - now);
+        ftop[h] = now;
+        fsum[h] *= c;
+#pragma unroll
+        for (int j = 0; j < (FEW > 0 ? NC : 1); ++j) fo[h][j] *= c;
+      }
+      const float p0 = __builtin_amdgcn_exp2f(x[h][0] - ftop[h]), p1 = __builtin_amdgcn_exp2f(x[h][1] - ftop[h]);
+      fsum[h] += p0 + p1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[h][i] = __shfl(i < 4 ? p0 : p1, 4 * g + (i & 3), 64);
+    }
+#pragma unroll
+    for (int part = 0; part < NP; ++part) {
+      auto& v = r.v[part & (NP > 1 ? 1 : 0)];
+      if (base + kTile > len) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (first + i >= len) {
+#pragma unroll
+            for (int c = 0; c < NV * EB / 4; ++c) v[i][c] = 0u;
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < NF; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            fo[h][part * NV + j] = fmaf(p[h][i], __uint_as_float(v[i][j]), fo[h][part * NV + j]);
+      if (NP > 1 && part + 2 < NP) load_v(v, part + 2);
+    }
+  };
+
   const int t0 = sp * per + w;
   if (t0 < t_end) {
     int ids = a.split == 1 ? sound(t0 * kTile + (lane & 31) <= last ? early : 0) : look(t0);
     for (int t = t0; t < t_end; t += W) {
       point(t, ids);
-      compute(t, ids, t + W < t_end ? t + W : -1);
+      if constexpr (FEW > 0) compute_few(t, ids, t + W < t_end ? t + W : -1);
+      else compute(t, ids, t + W < t_end ? t + W : -1);
     }
   }
 
@@ -348,21 +450,42 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD)) paged_attn_kernel(Pa
     }
   }
 
-  sum += __shfl_xor(sum, 16, 64);
-  sum += __shfl_xor(sum, 32, 64);
-  if (__any(bad)) sum = NAN;
-  float* const lw = lds + (NP > 1 ? KL * 256 : 0);  // [W][cols][HD]
+  constexpr int kQ = FEW > 0 ? FEW * KL * 16 : NP > 1 ? KL * 256 : 0;  // (launch_one)
+  float* const lw = lds + kQ;              // [W][cols][HD]
   float* const lo = lw + w * cols * HD;
-  float* const lms = lw + W * cols * HD;            // [W][cols] maxima, then sums
-  if (m16 < cols) {
-    if (g == 0) {
-      lms[w * cols + m16] = top;
-      lms[(W + w) * cols + m16] = sum;
+  float* const lms = lw + W * cols * HD;   // [W][cols] maxima, then sums
+  const bool any_bad = __any(bad);
+  if constexpr (FEW > 0) {
+#pragma unroll
+    for (int h = 0; h < NF; ++h) {
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) fsum[h] += __shfl_xor(fsum[h], d, 64);
+      if (h < cols && lane == 0) {
+        lms[w * cols + h] = ftop[h];
+        lms[(W + w) * cols + h] = any_bad ? NAN : fsum[h];
+      }
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        float c = fo[h][j];
+        c += __shfl_xor(c, 16, 64);
+        c += __shfl_xor(c, 32, 64);
+        if (h < cols && g == 0) lo[h * HD + v_col<T, HD>(m16, j)] = c;
+      }
     }
+  } else {
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (any_bad) sum = NAN;
+    if (m16 < cols) {
+      if (g == 0) {
+        lms[w * cols + m16] = top;
+        lms[(W + w) * cols + m16] = sum;
+      }
 #pragma unroll
-    for (int j = 0; j < NC; ++j)
+      for (int j = 0; j < NC; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) lo[m16 * HD + v_col<T, HD>(4 * g + r, j)] = o[j][r];
+        for (int r = 0; r < 4; ++r) lo[m16 * HD + v_col<T, HD>(4 * g + r, j)] = o[j][r];
+    }
   }
   __syncthreads();
   for (int x = tid; x < cols * HD; x += W * 64) {
@@ -430,26 +553,38 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnArgs a) {
   }
 }
 
-template <DecodeType T, int HD, int W>
+template <DecodeType T, int HD, int W, int FEW>
 void launch_one(const PagedAttnArgs& a, hipStream_t stream) {
   const int group = a.heads / a.kv_heads, cols = group < 16 ? group : 16;
   typedef Tile<T, HD> Regs;
-  const uint32_t lds = static_cast<uint32_t>(W * cols * (HD + 2) * 4 + (Regs::NP > 1 ? Regs::KL * 1024 : 0));
+  const uint32_t lds = static_cast<uint32_t>(W * cols * (HD + 2) * 4 + (FEW > 0 ? FEW * Regs::KL * 64 : Regs::NP > 1 ? Regs::KL * 1024 : 0));
   if (lds > 65536)  // (of the current device: set wherever it is needed)
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, HD, W>),
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, HD, W, FEW>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
   const uint32_t blocks = static_cast<uint32_t>(a.n) * a.kv_heads * ((group + 15) / 16) * a.split;
-  COMMEFF_LAUNCH((paged_attn_kernel<T, HD, W>), dim3(blocks), dim3(W * 64), lds, stream, a);
+  COMMEFF_LAUNCH((paged_attn_kernel<T, HD, W, FEW>), dim3(blocks), dim3(W * 64), lds, stream, a);
   if (a.split > 1)
     COMMEFF_LAUNCH(paged_attn_join_kernel<T>, dim3(static_cast<uint32_t>(a.n) * a.heads), dim3(256), 0, stream, a);
+}
+
+template <DecodeType T, int HD, int W>
+void launch_group(const PagedAttnArgs& a, hipStream_t stream) {
+  if constexpr (T == kF32) {
+    if (a.group == 1) return launch_one<T, HD, W, 1>(a, stream);
+    if constexpr (HD <= 128) {  // (a second head of 256 columns does not fit the registers)
+      if (a.group == 2) return launch_one<T, HD, W, 2>(a, stream);
+    }
+  }
+  launch_one<T, HD, W, 0>(a, stream);
 }
 
 template <DecodeType T, int HD>
 void launch_dim(const PagedAttnArgs& a, hipStream_t stream) {
   if constexpr (HD * Tile<T, HD>::E <= 256) {
-    if (a.waves == 8) return launch_one<T, HD, 8>(a, stream);
+    if (a.waves == 8) return launch_group<T, HD, 8>(a, stream);
   }
-  launch_one<T, HD, 4>(a, stream);
+  if (a.waves == 1) return launch_group<T, HD, 1>(a, stream);
+  launch_group<T, HD, 4>(a, stream);
 }
 
 template <DecodeType T>
@@ -464,17 +599,20 @@ void launch_type(const PagedAttnArgs& a, hipStream_t stream) {
 
 // Waves a workgroup and parts a sequence.  A workgroup serves one (sequence,
 // cache head, 16 query heads), its waves take the sequence's tiles in turn: 8
-// of them, 4 where sequences are short (one or two tiles a wave: 64 x 12 heads
-// of up to 256 tokens 10.7 against 12.0 us) or rows fill the registers.  Where
-// there are fewer than 1,024 workgroups, a sequence of 6 or more tiles a wave
-// is split so that two are left: 1 x 12 heads, 4,096 tokens 11.5 against 29.7
-// us, 8 x 8 heads, 65,536 tokens 245 against 776; below that the second launch
-// costs more than it saves (16 x 12 heads, 1,024 tokens 15.5 against 11.9).
+// of them; 4 where sequences are short (64 x 12 heads of up to 256 tokens 10.7
+// against 12.0 us) or rows fill the registers; 1 for one or two tiles, or for
+// up to four where the batch fills the chip even so (250 x 12 heads, 32 tokens
+// 7.3 against 12.4 us, 128 tokens 14.0 against 16.4; 64 x 12 heads, 128 tokens
+// 9.7 against 7.6).  Where there are fewer than 1,024 workgroups, a sequence of
+// 6 or more tiles a wave is split so that two are left: 1 x 12 heads, 4,096
+// tokens 11.5 against 29.7 us, 8 x 8 heads, 65,536 tokens 245 against 776;
+// below that the second launch costs more than it saves (16 x 12 heads, 1,024
+// tokens 15.5 against 11.9).
 void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest) {
   const int group = a.heads / a.kv_heads;
   const int64_t groups = static_cast<int64_t>(a.n) * a.kv_heads * ((group + 15) / 16);
   const int64_t tiles = (longest + kTile - 1) / kTile;
-  a.waves = tiles > 8 && a.dim * (t == kF32 ? 4 : 2) <= 256 ? 8 : 4;
+  a.waves = tiles <= 2 || (tiles <= 4 && groups >= 2048) ? 1 : tiles > 8 && a.dim * (t == kF32 ? 4 : 2) <= 256 ? 8 : 4;
   int64_t split = 1;
   if (groups > 0 && tiles >= 6 * a.waves) split = (1024 + groups - 1) / groups;
   const int64_t most = tiles / (2 * a.waves);

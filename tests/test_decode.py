@@ -482,13 +482,15 @@ def _select_case(name):
         x[5, 1, 77] = 0.0
         x[6, :, 100:] = -INF
         return x.to(BF), rnd(40, 4).mul(8).round() / 8 + torch.arange(4) / 3, 16, None, -1
+    if name == "short":  # fewer 16-byte pieces than places
+        return rnd(5, 16, 401).to(BF), rnd(5, 16), 64, None, -1
     if name == "huge":
         return rnd(1, 2, 250007), rnd(1, 2), 4, None, -1
     raise KeyError(name)
 
 
 @pytest.mark.parametrize("name", ["one", "few", "odd", "wide", "padded", "unaligned", "columns", "first", "equal",
-                                  "steps", "masked", "dead", "finished", "spread", "sorted", "batch", "huge"])
+                                  "steps", "masked", "dead", "finished", "spread", "sorted", "batch", "short", "huge"])
 @pytest.mark.parametrize("device", DEVICES)
 def test_select(device, name):
     """Scores are off by fp32's rounding of the result and, on the GPU, by a log of a sum
