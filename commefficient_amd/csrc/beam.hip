@@ -104,7 +104,11 @@ __device__ __forceinline__ Best block_best(Best x, Best* lds) {
   return x;
 }
 
-// part `blockIdx.x` of row `blockIdx.y`: (maximum, sum of exponentials beside
+// 64 x 8 rows of 50,262 bf16 logits, a quarter of them at their end: 18 us for
+// 39 MB, bound by instructions (about 45 cycles an element and wave: unpack
+// twice, maximum, difference, exp at a quarter of the rate, sum, compare); four
+// rows 7 us, a chain of loads, a search and a list.
+// Part `blockIdx.x` of row `blockIdx.y`: (maximum, sum of exponentials beside
 // it) into stat, the best `keep` as ordered(logit) << 32 | ~index into cand, in
 // their order, 0 where there are fewer
 template <DecodeType T>
@@ -265,8 +269,9 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
 }
 
 // a request's beams: their log-sum-exp, the scores of what the parts kept, and
-// the best of them.  Bound by latency: the first candidates are on their way
-// while the sums are joined (a wave a beam), and stay in registers.
+// the best of them.  Bound by latency (one request of 4 beams 4.2 us, 64 of 8
+// beams 7.0): the first candidates are on their way while the sums are joined
+// (a wave a beam), and stay in registers.
 __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   constexpr int kHeld = 4;  // candidates a thread holds
   __shared__ Best s_list[kJoinList];

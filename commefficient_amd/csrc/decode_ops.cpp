@@ -105,6 +105,15 @@ at::Tensor unit_rows(const at::Tensor& x) {
   return x.size(2) == 1 || x.stride(2) == 1 ? x : x.contiguous();
 }
 
+// contiguous `size` elements of `buf` from `at` on: a narrow() without the
+// dispatcher, which would be half of such a call's host time
+at::Tensor piece_of(const at::Tensor& buf, int64_t at, at::IntArrayRef size) {
+  auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+  t->set_storage_offset(at);
+  t->set_sizes_contiguous(size);
+  return at::Tensor(std::move(t));
+}
+
 // ------------------------------------------------------------------ extend
 std::vector<at::Tensor> extend_outputs(at::Tensor& table, at::Tensor& lens, const at::Tensor& fresh,
                                        const at::Tensor& pool, at::Tensor& used, int64_t page, int64_t rows,
@@ -124,12 +133,10 @@ std::vector<at::Tensor> extend_outputs(at::Tensor& table, at::Tensor& lens, cons
   const int64_t all = 2 * (rows + 3) + n + 1 + 3 + 4 + (in_place ? 0 : n + 3 + 4);
   const auto buf = at::empty({all}, i32);
   int64_t at = 0;
-  auto piece = [&](int64_t size) {  // (a narrow() without the dispatcher: half of this call's host time otherwise)
-    auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
-    t->set_storage_offset(at);
-    t->set_sizes_contiguous({size});
+  auto piece = [&](int64_t size) {
+    auto t = piece_of(buf, at, {size});
     at += (size + 3) / 4 * 4;  // (each at a multiple of 16 bytes)
-    return at::Tensor(std::move(t));
+    return t;
   };
   std::vector<at::Tensor> out;
   out.reserve(7);
@@ -532,8 +539,8 @@ void check_select(const at::Tensor& logits, const at::Tensor& scores, int64_t ke
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> select_outputs(const at::Tensor& scores, int64_t keep) {
   const int64_t b = scores.size(0);
-  auto ids = at::empty({2, b, keep}, scores.options().dtype(at::kLong));
-  return {at::empty({b, keep}, scores.options()), ids.select(0, 0), ids.select(0, 1)};
+  const auto ids = at::empty({2 * b * keep}, scores.options().dtype(at::kLong));
+  return {at::empty({b, keep}, scores.options()), piece_of(ids, 0, {b, keep}), piece_of(ids, b * keep, {b, keep})};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_hip(const at::Tensor& logits, const at::Tensor& scores,

@@ -20,7 +20,9 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 // + p % page.  A few hundred KB at most: bound by latency, that is by the
 // launch, two scans and the chain row -> sequence -> page.  So one workgroup
 // does all of it with the sequences' plan in LDS; only batches too large for
-// that (kFused) leave the rows to a second launch over the whole chip.
+// that (kFused) leave the rows to a second launch over the whole chip.  16
+// prompts of up to 500 tokens 7.1 us (an empty launch 1.4, the scans 2.8, the
+// rows 2.9), one token for 4,096 sequences 11.1.
 constexpr int kScan = 1024, kEach = 4;  // threads of the scan, sequences a thread takes at once
 constexpr int kFused = 8192;            // sequences and rows of a single launch
 

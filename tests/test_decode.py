@@ -692,6 +692,29 @@ def test_steps_captured_gpu():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,group,dim", [(BF, 16, 256), (FP, 16, 256), (FP, 1, 256), (BF, 1, 64)])
+def test_attention_captured_gpu(dtype, group, dim):
+    """Replays follow the lengths, tables and rows that they find (the first call of a variant
+    may be the captured one)."""
+    lens = [70, 33, 5]
+    q, k, v, kc, vc, table = _attention_case(dtype, lens, 1, group, dim, 16)
+    dev = [_on("cuda", x) for x in (q, kc, vc, table, torch.tensor(lens, dtype=torch.int32))]
+    kw = dict(k=k.cuda(), v=v.cuda())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = decode.paged_attention(*dev, **kw)
+    for now in ([70, 33, 5], [1, 32, 0], [64, 2, 4], [70, 33, 5]):
+        dev[0].copy_(torch.randn(q.shape, generator=_g(sum(now))).to(dtype))
+        dev[4].copy_(torch.tensor(now, dtype=torch.int32))
+        kc, vc = dev[1].cpu(), dev[2].cpu()
+        graph.replay()
+        torch.randn(1 << 14, device="cuda").sum().item()
+        want, bound = _attention_oracle(dev[0].cpu(), kc, vc, table, now, dim ** -0.5, k, v)
+        assert bool(((out.cpu().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.gpu
 def test_other_stream_gpu():
     """The operators run on the caller's current stream."""
     lens = [300, 17, 1024]
@@ -776,8 +799,9 @@ def test_generate_native_bf16_gpu():
     g = _g(6)
     prompts = [torch.randint(0, 50262, (n,), generator=g).tolist() for n in (16, 3, 50)]
     out = generate(m, prompts, max_new_tokens=12, num_beams=4)
+    out += generate(m, prompts[1:2], max_new_tokens=12, num_beams=1)
     ref = m.float()
-    for p, (tokens, score) in zip(prompts, out):
+    for p, (tokens, score) in zip(prompts + prompts[1:2], out):
         assert len(tokens) == 12
         with torch.no_grad():
             x = ref.lm_head(ref.transformer(torch.tensor([p + tokens], device="cuda"))[0][0])
