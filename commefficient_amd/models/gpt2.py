@@ -153,10 +153,10 @@ def generate(model, prompts, *, max_new_tokens=20, num_beams=4, eos=None, token_
     The reference evaluates perplexity and candidate ranking only
     (gpt2_train.py:149-253); replies follow its model and input format."""
     m = model.model if isinstance(model, GPT2DoubleHeads) else model
-    tr = m.transformer
-    cfg = tr.config
+    tr = getattr(m, "transformer", None)
+    cfg = getattr(tr, "config", None)
     if getattr(cfg, "model_type", "") != "gpt2":
-        raise ValueError("generate() covers GPT-2 models, not %r" % getattr(cfg, "model_type", None))
+        raise ValueError("generate() covers GPT-2 models, not %r" % getattr(cfg, "model_type", type(m).__name__))
     lens = [len(p) for p in prompts]
     if not lens:
         return []

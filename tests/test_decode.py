@@ -819,8 +819,28 @@ def test_generate_refusals():
         with pytest.raises(ValueError):
             generate(m, **kw)
     o = build_double_heads("openai-gpt", n_special=0, n_layer=1, n_embd=32, n_head=2)
-    with pytest.raises(ValueError, match="GPT-2"):
-        generate(o, [[1]])
+    for other in (o, torch.nn.Linear(2, 2)):
+        with pytest.raises(ValueError, match="GPT-2"):
+            generate(other, [[1]])
+
+
+@pytest.mark.parametrize("dtype,device", [(BF, "cpu"), pytest.param(HF, "cuda", marks=pytest.mark.gpu),
+                                          pytest.param(BF, "cuda", marks=pytest.mark.gpu)])
+def test_generate_other_types(dtype, device):
+    """Models that the native junctions do not cover (fp16, 64 columns) answer too: as many
+    tokens as asked for, of the vocabulary, with the score of the HF forward of the same
+    tokens (16-bit hidden states: logits of up to ~30 rounded to 2^-4)."""
+    m = _tiny(64, 2, dtype, device)
+    prompts = [[11, 7000, 42], [50000]]
+    for p, (tokens, score) in zip(prompts, generate(m, prompts, max_new_tokens=5, num_beams=2, page_size=2)):
+        assert len(tokens) == 5 and all(0 <= t < 50262 for t in tokens)
+        with torch.no_grad():
+            ref = m.float()
+            x = ref.lm_head(ref.transformer(torch.tensor([p + tokens], device=device))[0][0])
+            m.to(dtype)
+        lp = torch.log_softmax(x.double(), 1)[len(p) - 1:-1]
+        s = float(lp.gather(1, torch.tensor(tokens, device=device)[:, None]).mean())
+        assert abs(s - score) < 0.25, (s, score)
 
 
 # ------------------------------------------------------------------- driver
