@@ -297,8 +297,10 @@ def test_attention(device, dtype, lens, kv_heads, group, dim, page, layout, appe
                 wk[table[i, (n - 1) // page], :, (n - 1) % page] = k[i]
                 wv[table[i, (n - 1) // page], :, (n - 1) % page] = v[i]
     dk, dv = _on(device, kc), _on(device, vc)
-    for hint in (None, 1):
-        out = decode.paged_attention(_on(device, q), dk, dv, table.to(device),
+    wide = torch.full((len(lens), table.shape[1] + 3), 1 << 30, dtype=torch.int32)  # rows further apart
+    wide[:, :table.shape[1]] = table
+    for hint, t in ((None, table.to(device)), (1, wide.to(device)[:, :table.shape[1]])):
+        out = decode.paged_attention(_on(device, q), dk, dv, t,
                                      torch.tensor(lens, dtype=torch.int32, device=device),
                                      k=_on(device, k) if append else None, v=_on(device, v) if append else None,
                                      max_len=hint)
@@ -552,6 +554,8 @@ def test_reorder(device, strided, dtype, requests, beams, layers, heads, page, d
     if strided:
         kv = kv.permute(2, 0, 1, 4, 3, 5).contiguous().permute(1, 2, 0, 4, 3, 5)
     t, c = table.to(device), _on(device, kv)
+    if strided:
+        t = torch.cat([t, torch.full_like(t, -5)], 1)[:, :width]
     decode.beam_reorder(parent.to(device), t, full.to(device), c)
     assert torch.equal(t.cpu(), want_t)
     assert torch.equal(c.cpu(), want)
