@@ -23,9 +23,11 @@
 // So K and V go from memory to the matrix cores without LDS.  Weights are fed
 // as two 16-bit pieces (a rounding and its remainder: 2^-16 of a weight for
 // bf16, 2^-22 for fp16), sums and maxima stay in fp32; fp32 caches use the
-// fp32 MFMA.  The running maximum is only raised when some score exceeds it
-// by kSlack (in powers of two), which a wave votes on: the cross-lane maximum
-// and the rescaling of O run a few times a sequence, not once a tile.
+// fp32 MFMA.  A wave whose sums come out infinite or NaN takes its tiles a second
+// time, so that an infinite value meets its weight once and not in two pieces.
+// The running maximum is only raised when some score exceeds it by kSlack (in
+// powers of two), which a wave votes on: the cross-lane maximum and the rescaling
+// of O run a few times a sequence, not once a tile.
 // Reached: 8 sequences of up to 65,536 tokens, 32 heads over 8 of 128, bf16:
 // 1.21 GB at 5.0 TB/s; 128 x 8 heads of 128, up to 1,024 tokens: 271 MB at 4.6;
 // 64 x 12 of 64: 103 MB in 27 us, 7 of them start and end; one short reply 6.
@@ -45,12 +47,18 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 constexpr int kTile = 32;       // tokens a wave takes at a time
 constexpr int kMaxSplit = 64;   // parts of a sequence
 
+template <bool B>
+struct Flag {
+  static constexpr bool value = B;
+};
+
 template <DecodeType T>
 struct Elem;
 template <>
 struct Elem<kBf16> {
   typedef uint16_t t;
   static constexpr float kSlack = 8.f, kLift = 0.f;
+  static constexpr uint32_t kExp = 0x7f80u, kUlp = 0x0080u;  // an exponent's bits, the lowest of them
   static __device__ __forceinline__ t store(float f) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f)); }
   static __device__ __forceinline__ float load(t x) { return bf2f(x); }
   static __device__ __forceinline__ f32x4_t mfma(v4u a, v4u b, f32x4_t c) {
@@ -63,6 +71,7 @@ struct Elem<kF16> {
   typedef uint16_t t;
   // weights reach 2^(1 + 12) < 65,504 and the smallest kept piece is 2^-24 / 2^12
   static constexpr float kSlack = 1.f, kLift = 12.f;
+  static constexpr uint32_t kExp = 0x7c00u, kUlp = 0x0400u;
   static __device__ __forceinline__ t store(float f) {
     return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
   }
@@ -106,6 +115,32 @@ template <DecodeType T, int HD>
 __device__ __forceinline__ int v_col(int m, int j) {
   constexpr int CH = Tile<T, HD>::CH;
   return (j / CH) * (16 * CH) + m * CH + j % CH;
+}
+
+// What of a lane's V pieces is infinite or NaN, times the weights' first pieces, into o; the
+// pieces keep the rest.  One dword (two columns) after the other: no registers for all.
+template <DecodeType T, int N>
+__device__ __forceinline__ void take_odd(uint32_t (&v)[8][N], v4u hi, f32x4_t* o) {
+  typedef Elem<T> E;
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    uint32_t odd[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      asm volatile("" : "+v"(v[i][c]));
+      // (an exponent of all ones and one more: the half's sign bit)
+      odd[i] = v[i][c] & ((((v[i][c] & (E::kExp * 0x10001u)) + E::kUlp * 0x10001u) >> 15 & 0x10001u) * 0xffffu);
+      v[i][c] ^= odd[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      v4u vt;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        vt[i] = __builtin_amdgcn_perm(odd[2 * i + 1], odd[2 * i], j ? 0x07060302u : 0x05040100u);
+      o[2 * c + j] = E::mfma(vt, hi, o[2 * c + j]);
+    }
+  }
 }
 
 // FEW > 0 (fp32, groups of FEW = 1 or 2 heads): the products on the
@@ -269,7 +304,11 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD, FEW)) paged_attn_kern
     }
     return c;
   };
-  auto compute = [&](int tile, int& ids, int next) {
+  // `flag`, careful: infinite and NaN values enter beside the first piece of their weight alone (0
+  // where the weight is: 0 x inf is NaN, as in fp32), the finite ones as ever.  The second,
+  // which may be 0 or negative, would make an infinity NaN.
+  auto compute = [&](int tile, int& ids, int next, auto flag) {
+    constexpr bool careful = decltype(flag)::value;
     Regs r;
     const int first = tile * kTile + 8 * g;
     f32x4_t s4[2];
@@ -314,6 +353,8 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD, FEW)) paged_attn_kern
         const uint32_t u0 = E::store(p[2 * i]), u1 = E::store(p[2 * i + 1]);
         hi[i] = u0 | u1 << 16;
         lo[i] = E::store(p[2 * i] - E::load(u0)) | static_cast<uint32_t>(E::store(p[2 * i + 1] - E::load(u1))) << 16;
+        if constexpr (T == kF16 && careful)  // (2^-36 of the largest for weights too small for fp16)
+          hi[i] |= (u0 == 0 && p[2 * i] != 0.f ? 1u : 0u) | (u1 == 0 && p[2 * i + 1] != 0.f ? 0x10000u : 0u);
       }
     }
 #pragma unroll
@@ -327,6 +368,7 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD, FEW)) paged_attn_kern
             for (int c = 0; c < NV * EB / 4; ++c) v[i][c] = 0u;
           }
       }
+      if constexpr (T != kF32 && careful) take_odd<T>(v, hi, o + part * NV);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         f32x4_t& oj = o[part * NV + j];
@@ -432,12 +474,31 @@ __global__ void __launch_bounds__(W * 64, min_waves(T, HD, FEW)) paged_attn_kern
   };
 
   const int t0 = sp * per + w;
-  if (t0 < t_end) {
+  auto sweep = [&](auto flag) {
     int ids = a.split == 1 ? sound(t0 * kTile + (lane & 31) <= last ? early : 0) : look(t0);
     for (int t = t0; t < t_end; t += W) {
       point(t, ids);
       if constexpr (FEW > 0) compute_few(t, ids, t + W < t_end ? t + W : -1);
-      else compute(t, ids, t + W < t_end ? t + W : -1);
+      else compute(t, ids, t + W < t_end ? t + W : -1, flag);
+    }
+  };
+  if (t0 < t_end) {
+    sweep(Flag<false>{});
+    if constexpr (T != kF32) {
+      // Once more, carefully, where a sum is not finite: rare, and a test of every value would
+      // cost the others 4 % (64 x 12 heads of 64: 28.0 against 26.7 us).
+      float z[4] = {0.f, 0.f, 0.f, 0.f};  // 0, or NaN
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[r] = fmaf(o[j][r], 0.f, z[r]);
+      const float odd = (z[0] + z[1]) + (z[2] + z[3]);
+      if (__any(m16 < cols && odd != 0.f)) {
+        top = -FLT_MAX, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        sweep(Flag<true>{});
+      }
     }
   }
 

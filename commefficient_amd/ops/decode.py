@@ -81,9 +81,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     [sequences, kv heads, head dim], the last of the ``lens`` tokens is the new one:
     its rows are read from there and stored into its slot by the same launch (a
     slot that no other sequence of the call reads or stores).  Rows of sequences
-    without tokens, or with no score above -inf, are 0.  A row is NaN where the table names a page outside the cache (nothing is read
-    through it) or is too short for ``lens``.  ``max_len`` (host) is a hint of the
-    longest sequence, for the split of the work alone."""
+    without tokens, or with no score above -inf, are 0.  A row is NaN where the table
+    names a page outside the cache (nothing is read through it) or is too short for
+    ``lens``.  An infinite value makes its column of the row infinite, and NaN where
+    its weight is 0 in fp32 or the sum holds both infinities; finite values below
+    2^120 / tokens leave the sums finite.  ``max_len`` (host) is a hint of the longest
+    sequence, for the split of the work alone."""
     return _ops().paged_attention(q, k_cache, v_cache, table, lens, k, v, scale, max_len)
 
 

@@ -1,0 +1,127 @@
+"""Generation from a paged key-value cache where it meets its edges: infinite values,
+beams that tie, models that are not configured as GPT-2 is, overlapping caches, sizes at
+the launches' limits, and the kernel variants that groups of fp32 heads take."""
+import itertools
+import math
+
+import pytest
+import torch
+
+from commefficient_amd.ops import decode
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+U = 2.0 ** -24  # half a step of fp32
+INF, NAN = math.inf, math.nan
+
+
+def _g(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---------------------------------------------------------------- attention
+def _cache(dtype, lens, kv_heads, group, dim, page, seed):
+    """Random q, k and v caches and tables; pages in a random order."""
+    g = _g(seed)
+    need = [-(-n // page) for n in lens]
+    ids = torch.randperm(sum(need) + 1, generator=g).int()
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+    for i, n in enumerate(need):
+        table[i, :n] = ids[sum(need[:i]):sum(need[:i + 1])]
+    rnd = lambda *s: torch.randn(*s, generator=g).to(dtype)  # noqa: E731
+    return rnd(len(lens), kv_heads * group, dim), rnd(len(ids), kv_heads, page, dim), \
+        rnd(len(ids), kv_heads, page, dim), table
+
+
+def _attention(q, kc, vc, table, lens, scale):
+    """(out, bound) in 64 bits, every product on its own so that infinities act as IEEE says.
+
+    bound: a score is a sum of ``dim`` exact products in fp32 and a scale, off by at most
+    dx = (dim + 2) U scale max sum|q k|; its weight by 2 dx and 32 U for exp2 and the powers' argument,
+    the sums of L weights by L U, two 16-bit pieces of a weight by 2^-16 (bf16) and 2^-22 (fp16,
+    and 2^-35 where a weight is below 2^-24); one rounding of the result at the end."""
+    heads, dim = q.shape[1:]
+    kh, page = kc.shape[1:3]
+    out, bound = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    pieces = {BF: 2.0 ** -16, HF: 2.0 ** -22, FP: 0.0}[q.dtype]
+    for i, n in enumerate(lens):
+        ids = table[i, :-(-n // page)].long()
+        k, v = (c[ids].transpose(1, 2).reshape(-1, kh, dim)[:n].double() for c in (kc, vc))
+        for h in range(heads):
+            c = h // (heads // kh)
+            x = (k[:, c] * q[i, h].double()).sum(1) * scale
+            p = torch.softmax(x, 0)
+            out[i, h] = (p[:, None] * v[:, c]).sum(0)
+            dx = float((k[:, c] * q[i, h].double()).abs().sum(1).max()) * scale * (dim + 2) * U
+            size = v[:, c].abs().nan_to_num(0.0, 0.0, 0.0)
+            bound[i, h] = (2 * dx + (n + 32) * U + pieces) * (p @ size)
+            if q.dtype == HF:
+                bound[i, h] += 2.0 ** -35 * size.sum(0)
+    return out, bound + out.abs().nan_to_num(0.0, 0.0, 0.0) * (torch.finfo(q.dtype).eps / 2) + 1e-30
+
+
+def _close(got, want, bound):
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    odd = ~want.isfinite()
+    assert torch.equal(got[odd].nan_to_num(0.5), want[odd].nan_to_num(0.5))
+    err = torch.where(odd, 0.0, (got - want).abs())
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("dtype,kv_heads,group,dim,page", [
+    (BF, 2, 1, 64, 16), (HF, 2, 1, 64, 16), (BF, 1, 4, 128, 8), (HF, 1, 20, 32, 3), (BF, 1, 2, 256, 16),
+    (HF, 1, 3, 256, 1), (FP, 1, 1, 64, 16), (FP, 1, 3, 64, 4)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_infinite_values(device, dtype, kv_heads, group, dim, page):
+    """A value that is infinite makes its column infinite whatever its weight, two of opposite
+    signs or a NaN make it NaN, and no other column, head or sequence changes."""
+    lens = [70, 1, 33, 64, 300]
+    q, kc, vc, table = _cache(dtype, lens, kv_heads, group, dim, page, seed=dim + page)
+    at = lambda i, t: (table[i, t // page].long(), slice(None), t % page)  # noqa: E731
+    for i, t, col, x in ((0, 3, 0, INF), (0, 69, 1, -INF), (0, 5, 2, INF), (0, 6, 2, -INF), (0, 40, dim - 1, NAN),
+                         (0, 41, dim - 2, INF), (0, 42, dim - 2, INF), (1, 0, 7, INF), (1, 0, 8, -INF),
+                         (3, 63, 5, -INF), (4, 0, 1, INF), (4, 299, 1, INF), (4, 128, dim // 2, NAN),
+                         (4, 200, dim // 2 + 1, -INF)):
+        page_at, _, off = at(i, t)
+        vc[page_at, :, off, col] = x
+    q[1] = 0.0
+    want, bound = _attention(q, kc, vc, table, lens, dim ** -0.5)
+    assert want[1, :, 7].eq(INF).all() and want[0, :, 2].isnan().all()
+    out = decode.paged_attention(q.to(device), kc.to(device), vc.to(device), table.to(device),
+                                 torch.tensor(lens, dtype=torch.int32, device=device))
+    _close(out, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_infinite_values_beside_weights_of_all_kinds(device, dtype):
+    """Weights that 16 bits hold exactly, that they round up or down, equal ones, and the new
+    token's row; a weight of exactly 0 beside an infinite value is NaN, as 0 x inf is."""
+    dim, lens = 64, [1, 2, 8, 32, 77, 6]
+    q, kc, vc, table = _cache(dtype, lens, 1, 1, dim, 16, seed=9)
+    q.zero_()
+    q[3:5, 0, 0] = 1.0
+    q[5, 0, 1] = 1.0
+    for i, n in enumerate(lens):
+        for t in range(n):
+            vc[table[i, t // 16], 0, t % 16, t % dim] = INF if t % 3 else -INF
+    kc[table[5, 0], 0, 2, 1] = -INF  # (no weight, beside column 2's infinity)
+    want, bound = _attention(q, kc, vc, table, lens, 0.25)
+    assert want[5, 0, 2].isnan() and want[:5, 0, 0].eq(-INF).sum() == 4
+    k, v = (torch.stack([c[table[i, (n - 1) // 16], :, (n - 1) % 16] for i, n in enumerate(lens)]) for c in (kc, vc))
+    a = [x.to(device) for x in (q, kc, vc, table, torch.tensor(lens, dtype=torch.int32))]
+    _close(decode.paged_attention(*a, scale=0.25), want, bound)
+    _close(decode.paged_attention(*a, scale=0.25, k=k.to(device), v=v.to(device)), want, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_attention_infinite_values_of_a_split_sequence_gpu(dtype):
+    lens = [9000, 5000]
+    q, kc, vc, table = _cache(dtype, lens, 2, 1, 64, 16, seed=3)
+    for i, t, col, x in ((0, 8999, 4, INF), (0, 17, 9, -INF), (1, 4000, 4, NAN), (1, 100, 63, INF), (1, 4999, 63, -INF)):
+        vc[table[i, t // 16], 1, t % 16, col] = x
+    want, bound = _attention(q, kc, vc, table, lens, 0.125)
+    out = decode.paged_attention(*(x.cuda() for x in (q, kc, vc, table, torch.tensor(lens, dtype=torch.int32))))
+    _close(out, want, bound)
