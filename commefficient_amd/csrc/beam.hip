@@ -13,8 +13,19 @@
 // in fp32) in registers, takes
 // their maximum, the sum of exponentials beside it and the `keep` best of
 // them.  The second turns what is left of a request (beams x parts x keep)
-// into scores, in 64 bits: candidates of different beams may lie closer than
-// fp32 tells apart.
+// into scores.
+//
+// Candidates of different beams are in the order of 64 bits.  Scores are formed in
+// 64 bits, but the sums' exponentials are the hardware's: a term beside its wave's
+// maximum m is off by 2^-24 x (1 for x - m, 1.25 for its product with log2 e) |x - m|,
+// 2^-23 for exp2 (1.42 x 2^-24 at most, measured) and 3 x 2^-24 for the fp32 sum of a
+// 16-byte piece; everything above that is in 64 bits.  The mean of |x - m| under the
+// softmax is at most log(vocabulary) (entropy), so a log-sum-exp is off by at most
+// 2^-24 (5 + 2.25 log(vocabulary)).  Where two candidates of different beams, one of
+// them among the `keep` best, are closer than twice that (one request of 8 beams and 16
+// places in a thousand), the join sums those beams' rows again in 64 bits, by index, so
+// that equal rows give equal sums wherever they lie, and chooses anew: 17 us a row of
+// 50,262 logits, which other requests do not wait for.
 //
 // The best of many by a threshold: of the 64 lanes of a wave, at least `keep`
 // hold an element that is no less than the keep-th largest of the lanes' own
@@ -24,6 +35,7 @@
 // lists hold pass (thousands of equal logits) `keep` rounds of an argmax take over.
 #include <hip/hip_runtime.h>
 #include <cfloat>
+#include <cmath>
 #include <cstdint>
 #include "conv_common.h"
 #include "decode.h"
@@ -68,8 +80,7 @@ __device__ __forceinline__ double unordered(u64 u) {
 constexpr uint32_t kNone = 0x007fffffu;  // ordered(-inf): no candidate
 
 // a bound that at least `keep` lanes' values reach (0 where fewer than `keep`
-// lanes have any): the keep-th largest, or less by bits that do not matter;
-// two bits at a time, since a ballot's way to the next comparison is what costs
+// lanes have any): the keep-th largest, or less by bits that do not matter
 __device__ __forceinline__ uint32_t wave_bound(uint32_t x, int keep) {
   uint32_t bound = 0;
   for (int bit = 31; bit >= 0; --bit) {
@@ -108,14 +119,12 @@ __device__ __forceinline__ Best block_best(Best x, Best* lds) {
 // 39 MB, bound by the chain of its phases (loads, maxima, search, exponentials,
 // list, ranks): some 800 vector instructions a wave, a sixth of its life, and
 // neither fewer of them nor more waves a SIMD shorten it; four rows 7 us.
-// Part `blockIdx.x` of row `blockIdx.y`: (maximum, sum of exponentials beside
-// it) into stat, the best `keep` as ordered(logit) << 32 | ~index into cand, in
+// Part `blockIdx.x` of row `blockIdx.y`: every wave's (maximum, sum of exponentials
+// beside it) into stat, the best `keep` as ordered(logit) << 32 | ~index into cand, in
 // their order, 0 where there are fewer
 template <DecodeType T>
 __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
   constexpr int EB = T == kF32 ? 4 : 2, GE = 16 / EB;  // elements of 16 bytes
-  __shared__ float s_f[4];
-  __shared__ double s_d[4];
   __shared__ uint32_t s_u[4];
   __shared__ u64 s_list[4][kList];
   __shared__ Best s_best[4];
@@ -177,17 +186,26 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
   // the exponentials beside the wave's own maximum; the difference first, so
   // that its rounding is that of a small number.  NaN (+inf - inf too) stays.
   const float beside = fmaxf(m, -FLT_MAX);
-  float sum = 0.f;
+  double all = 0.0;
 #pragma unroll
   for (int i = 0; i < kPieces; ++i)
     if (i * kThreads < per) {  // (a whole piece of the workgroup: rows shorter than its registers)
+      float x[GE];
 #pragma unroll
-      for (int e = 0; e < GE; ++e) sum += __builtin_amdgcn_exp2f((at(i, e) - beside) * kLog2e);
+      for (int e = 0; e < GE; ++e) x[e] = __builtin_amdgcn_exp2f((at(i, e) - beside) * kLog2e);
+#pragma unroll
+      for (int o = 1; o < GE; o *= 2)
+#pragma unroll
+        for (int e = 0; e < GE; e += 2 * o) x[e] += x[e + o];
+      all += x[0];
     }
-  double all = sum;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, 64);
-  if (lane == 0) s_f[w] = m, s_u[w] = bound, s_d[w] = all;
+  if (lane == 0) {  // (a NaN: no row at all)
+    double* stat = a.stat + ((static_cast<int64_t>(row) * a.parts + part) * kBeamWaves + w) * 2;
+    stat[0] = all != all ? INFINITY : m, stat[1] = all;
+    s_u[w] = bound;
+  }
   if (a.tight) {  // the waves' best lanes together: a bound for all four
     const u64 mask = __ballot(ordered(most + 0.f) >= bound);
     const int c = __popcll(mask & ((1ull << lane) - 1));
@@ -195,21 +213,9 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
     if ((mask >> lane & 1) && c < 16) s_v[w * 16 + c] = ordered(most + 0.f);
   }
   __syncthreads();
-  m = fmaxf(fmaxf(s_f[0], s_f[1]), fmaxf(s_f[2], s_f[3]));
   bound = max(max(max(s_u[0], s_u[1]), max(s_u[2], s_u[3])), kNone + 1);
   if (a.tight) bound = max(bound, wave_bound(s_v[lane], a.keep));
-  all = 0.0;
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i)
-    all += s_d[i] * __builtin_amdgcn_exp2f((fmaxf(s_f[i], -FLT_MAX) - fmaxf(m, -FLT_MAX)) * kLog2e);
-  double* stat = a.stat + (static_cast<int64_t>(row) * a.parts + part) * 2;
   u64* cand = a.cand + (static_cast<int64_t>(row) * a.parts + part) * a.keep;
-  if (!(fabsf(m) < INFINITY) || all != all) {  // nothing above -inf, or no row at all
-    if (tid == 0) stat[0] = all != all ? INFINITY : m, stat[1] = 0.0;
-    for (int k = tid; k < a.keep; k += kThreads) cand[k] = 0;
-    return;
-  }
-  if (tid == 0) stat[0] = m, stat[1] = all;
   auto key = [](float x, int v) {  // (-0 is +0)
     return static_cast<u64>(ordered(x + 0.f)) << 32 | (0xffffffffu - static_cast<uint32_t>(v));
   };
@@ -268,23 +274,76 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
   }
 }
 
+// exp(x), -701 <= x <= 0: 2^n e^r with n next to x / log 2 (the low bits of a sum that holds
+// no fraction), |r| < 0.35 and e^r its series to 4e-18; off by some 1e-15
+__device__ __forceinline__ double exp64(double x) {
+  constexpr double kLog2 = 0.69314718055994530942, kHi = 0x1.62e42fefap-1;  // (the upper part of log(2))
+  constexpr double kWhole = 0x1.8p52;
+  constexpr double kTerm[14] = {1.0, 1.0, 0.5, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
+                                1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600, 1.0 / 6227020800.0};
+  const double sum = fma(x, 1.0 / kLog2, kWhole), n = sum - kWhole;
+  const double r = fma(n, -(kLog2 - kHi), fma(n, -kHi, x));
+  double e = kTerm[13];
+#pragma unroll
+  for (int i = 12; i >= 0; --i) e = fma(e, r, kTerm[i]);
+  const u64 up = static_cast<u64>(static_cast<uint32_t>(__builtin_bit_cast(u64, sum))) << 52;
+  return __builtin_bit_cast(double, __builtin_bit_cast(u64, e) + up);  // (2^n into the exponent)
+}
+
+// a thread's part of a row's sum of exp(x - m): every 256th 16 bytes from the row's first
+// element on, whatever its alignment; seven loads on their way under the eighth's terms
+template <DecodeType T>
+__device__ __forceinline__ double row_sum(const BeamSelectArgs& a, int64_t at, double m) {
+  constexpr int EB = T == kF32 ? 4 : 2, GE = 16 / EB, kAhead = 8;
+  const unsigned char* p = static_cast<const unsigned char*>(a.logits) + at * EB;
+  const int full = a.vocab / GE, tid = threadIdx.x;
+  const float least = static_cast<float>(m) - 700.f;  // (-inf: e^-700 of the greatest term)
+  auto load = [&](int i) {
+    v4u u = {kLow<T>, kLow<T>, kLow<T>, kLow<T>};
+    if (i < full) __builtin_memcpy(&u, p + static_cast<int64_t>(i) * 16, 16);
+    return u;
+  };
+  v4u u[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) u[i] = load(tid + i * kThreads);
+  double sum = 0.0;
+  for (int i = tid; i < full; i += kThreads) {
+    const v4u now = u[0];
+#pragma unroll
+    for (int k = 0; k + 1 < kAhead; ++k) u[k] = u[k + 1];
+    u[kAhead - 1] = load(i + kAhead * kThreads);
+#pragma unroll
+    for (int e = 0; e < GE; ++e)
+      sum += exp64(fmaxf(to_float<T>(EB == 4 ? now[e % 4] : (now[e / 2] >> (16 * (e & 1))) & 0xffffu), least) - m);
+  }
+  const int v = full * GE + tid;
+  if (v < a.vocab) {
+    uint32_t x = 0;
+    __builtin_memcpy(&x, p + static_cast<int64_t>(v) * EB, EB);
+    sum += exp64(fmaxf(to_float<T>(x), least) - m);
+  }
+  return sum;
+}
+
 // a request's beams: their log-sum-exp, the scores of what the parts kept, and
-// the best of them.  Bound by latency (one request of 4 beams 4.2 us, 64 of 8
-// beams 7.0): the first candidates are on their way while the sums are joined
+// the best of them.  Bound by latency (one request of 4 beams 4.7 us, 64 of 8
+// beams 7.5): the first candidates are on their way while the sums are joined
 // (a wave a beam), and stay in registers.
 __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   constexpr int kHeld = 4;  // candidates a thread holds
-  __shared__ Best s_list[kJoinList];
+  __shared__ Best s_list[kJoinList], s_sorted[kJoinList];
   __shared__ Best s_best[4];
+  __shared__ double s_sum[4];
   __shared__ uint32_t s_u[2][4];
-  __shared__ int s_n;
+  __shared__ uint32_t s_again[kBeamMaxBeams / 32];  // a bit a beam: its sum in 64 bits
+  __shared__ int s_n, s_near;
   extern __shared__ __attribute__((aligned(16))) double s_lse[];  // [beams], +inf: no continuation by its logits
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t row0 = static_cast<int64_t>(b) * a.beams;
   auto ends = [&](int j) { return a.finished && a.finished[row0 + j]; };
   auto alive = [&](int j) { return !ends(j) && fabsf(a.scores[row0 + j]) < INFINITY; };
   // candidate c: the (c / lists)-th of list c % lists, so that a wave's lanes see the lists' heads
-  const int lists = a.beams * a.parts, all = lists * a.keep;
+  const int lists = a.beams * a.parts, all = lists * a.keep, stats = a.parts * kBeamWaves;
   auto place = [&](int c, int& rank, int& list, int& j) {
     rank = a.by_lists.of(c);
     list = c - rank * lists;
@@ -298,37 +357,50 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   u64 held[kHeld];
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) held[i] = tid + i * kThreads < all ? fetch(tid + i * kThreads) : 0;
+  double size = 0.0;  // of what a score is formed from
   for (int j = w; j < a.beams; j += kThreads / 64) {
     double lse = INFINITY;
-    const double* stat = a.stat + (row0 + j) * a.parts * 2;
+    const double* stat = a.stat + (row0 + j) * stats * 2;
     double m = -INFINITY, sum = 0.0;
-    for (int i = lane; i < a.parts; i += 64) m = fmax(m, stat[2 * i]);
+    for (int i = lane; i < stats; i += 64) m = fmax(m, stat[2 * i]);
     if (alive(j)) {
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
       if (fabs(m) < INFINITY) {
-        for (int i = lane; i < a.parts; i += 64)
+        for (int i = lane; i < stats; i += 64)
           if (stat[2 * i + 1] > 0.0) sum += stat[2 * i + 1] * exp(stat[2 * i] - m);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         lse = m + log(sum);
+        size = fmax(size, fabs(lse) + fabsf(a.scores[row0 + j]));
       }
     }
     if (lane == 0) s_lse[j] = lse;
   }
-  if (tid == 0) s_n = 0;
+  if (lane == 0) s_sum[w] = size;
+  if (tid < kBeamMaxBeams / 32) s_again[tid] = 0;
+  if (tid == 0) s_n = s_near = 0;
   __syncthreads();
-  auto score = [&](int c, u64 k) {  // value 0: none
+  // closer than this: the order is not certain (64-bit roundings of large scores, too)
+  const double near = a.near + 0x1p-50 * fmax(fmax(s_sum[0], s_sum[1]), fmax(s_sum[2], s_sum[3]));
+  auto score = [&](int c, u64 k) {  // value 0: none; index: beam << 32 | token
     int rank, list, j;
     place(c, rank, list, j);
     const double s = a.scores[row0 + j];
+    const u64 beam = static_cast<u64>(j) << 32;
     if (ends(j)) {
       if (rank != 0 || list != j * a.parts || !(fabs(s) < INFINITY)) return Best{0, 0};
-      return Best{ordered(s + 0.0), static_cast<u64>(j) * a.vocab + a.eos};
+      return Best{ordered(s + 0.0), beam | static_cast<u64>(a.eos)};
     }
     if (k == 0 || s_lse[j] == INFINITY) return Best{0, 0};
     const double x = s + (unordered(static_cast<uint32_t>(k >> 32)) - s_lse[j]);
-    return Best{ordered(x + 0.0), static_cast<u64>(j) * a.vocab + (0xffffffffu - static_cast<uint32_t>(k))};
+    return Best{ordered(x + 0.0), beam | (0xffffffffu - static_cast<uint32_t>(k))};
+  };
+  auto put = [&](int k, const Best& x, bool some) {
+    const int64_t at = static_cast<int64_t>(b) * a.keep + k;
+    a.out_scores[at] = some ? static_cast<float>(unordered(x.value)) : -INFINITY;
+    a.out_parent[at] = some ? static_cast<int64_t>(x.index >> 32) : 0;
+    a.out_token[at] = some ? static_cast<int64_t>(x.index & 0xffffffffu) : 0;
   };
   Best mine[kHeld];
   uint32_t most = 0;  // the upper halves do for a bound
@@ -361,6 +433,11 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
       if (n == a.keep) break;
     }
   }
+  // (down to what may belong above it; up to 0x000fffff no number's upper half)
+  if (bound > 0x000fffffu) {
+    const double x = unordered(static_cast<u64>(bound) << 32);
+    bound = static_cast<uint32_t>(ordered(x - near - 0x1p-50 * fabs(x)) >> 32);
+  }
   bound = max(bound, 1u);
   auto pass = [&](const Best& x) {
     if (static_cast<uint32_t>(x.value >> 32) >= bound) {
@@ -373,14 +450,7 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   for (int c = tid + kHeld * kThreads; c < all; c += kThreads) pass(score(c, fetch(c)));
   __syncthreads();
   const int n = s_n;
-  auto put = [&](int k, const Best& x, bool some) {
-    const int64_t at = static_cast<int64_t>(b) * a.keep + k;
-    const int j = some ? static_cast<int>(x.index) / a.vocab : 0;  // (beams x vocabulary < 2^31)
-    a.out_scores[at] = some ? static_cast<float>(unordered(x.value)) : -INFINITY;
-    a.out_parent[at] = j;
-    a.out_token[at] = some ? static_cast<int>(x.index) - j * a.vocab : 0;
-  };
-  if (n <= kJoinList) {
+  auto rank_list = [&] {
     for (int c = tid >> 2; c < n; c += kThreads / 4) {
       const Best x = s_list[c];
       int rank = 0;
@@ -388,9 +458,61 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
       for (int i = tid & 3; i < n; i += 4) rank += before(s_list[i], x);
       rank += __shfl_xor(rank, 1, 64);
       rank += __shfl_xor(rank, 2, 64);
-      if ((tid & 3) == 0 && rank < a.keep) put(rank, x, true);
+      if ((tid & 3) == 0) s_sorted[rank] = x;
     }
-    for (int k = n + tid; k < a.keep; k += kThreads) put(k, Best{0, 0}, false);
+    __syncthreads();
+    for (int k = tid; k < a.keep; k += kThreads) put(k, k < n ? s_sorted[k] : Best{0, 0}, k < n);
+  };
+  if (n <= kJoinList) {
+    rank_list();
+    // Neighbours of different beams, one of them kept (or no further from the last
+    // one kept): any two that are close have such neighbours between them.
+    for (int i = tid; i + 1 < n; i += kThreads) {
+      const int jx = static_cast<int>(s_sorted[i].index >> 32), jy = static_cast<int>(s_sorted[i + 1].index >> 32);
+      if (jx == jy) continue;
+      const double v = unordered(s_sorted[min(i, a.keep - 1)].value), u = unordered(s_sorted[i + 1].value);
+      if (v - u <= near + 0x1p-50 * fabs(v)) {
+        s_near = 1;
+        atomicOr(&s_again[jx >> 5], 1u << (jx & 31));
+        atomicOr(&s_again[jy >> 5], 1u << (jy & 31));
+      }
+    }
+    __syncthreads();
+    if (s_near == 0) return;
+  } else if (a.beams > 1 && tid < kBeamMaxBeams / 32) {
+    s_again[tid] = ~0u;
+  }
+  __syncthreads();
+  // Rare: those beams' sums in 64 bits, and the list by them
+  for (int j = 0; j < a.beams; ++j) {
+    if (!(s_again[j >> 5] >> (j & 31) & 1) || !alive(j) || s_lse[j] == INFINITY) continue;
+    double m = -INFINITY;
+    for (int i = 0; i < stats; ++i) m = fmax(m, a.stat[((row0 + j) * stats + i) * 2]);
+    const int64_t at = b * a.s_request + j * a.s_beam;
+    double sum = 0.0;
+    if (a.type == kF32) sum = row_sum<kF32>(a, at, m);
+    else if (a.type == kBf16) sum = row_sum<kBf16>(a, at, m);
+    else sum = row_sum<kF16>(a, at, m);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) s_sum[w] = sum;
+    __syncthreads();
+    if (tid == 0) s_lse[j] = m + log(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
+    __syncthreads();
+  }
+  if (n <= kJoinList) {
+    for (int c = tid; c < n; c += kThreads) {
+      const int j = static_cast<int>(s_list[c].index >> 32);
+      if (ends(j)) continue;
+      const int64_t at = b * a.s_request + j * a.s_beam + static_cast<int64_t>(s_list[c].index & 0xffffffffu);
+      float x;
+      if (a.type == kF32) x = static_cast<const float*>(a.logits)[at];
+      else if (a.type == kBf16) x = to_float<kBf16>(static_cast<const uint16_t*>(a.logits)[at]);
+      else x = to_float<kF16>(static_cast<const uint16_t*>(a.logits)[at]);
+      s_list[c].value = ordered(a.scores[row0 + j] + (x - s_lse[j]) + 0.0);
+    }
+    __syncthreads();
+    rank_list();
     return;
   }
   Best last = {~0ull, 0};
@@ -426,6 +548,8 @@ void launch_beam_select(BeamSelectArgs a, DecodeType t, hipStream_t stream) {
   // where throughput counts (64 x 8 beams 24.6 against 26.6 us), not for few
   // workgroups (1 x 4 beams 11.6 against 11.1); its table holds 16 of a wave
   a.tight = a.keep <= 16 && static_cast<int64_t>(a.requests) * a.beams * a.parts >= 512;
+  a.type = t;
+  a.near = 2.0 * 0x1p-24 * (5.0 + 2.25 * std::log(static_cast<double>(a.vocab)));
   a.by_beams = fast_div(a.beams);
   a.by_parts = fast_div(a.parts);
   a.by_lists = fast_div(static_cast<int64_t>(a.beams) * a.parts);

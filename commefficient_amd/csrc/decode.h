@@ -35,6 +35,8 @@ inline FastDiv fast_div(int64_t d) {
 }
 
 constexpr int kBeamMaxKeep = 64;     // candidates of one beam_select request
+constexpr int kBeamMaxBeams = 1024;
+constexpr int kBeamWaves = 4;        // of a workgroup of its first kernel
 constexpr int kReorderMaxBeams = 32;
 
 struct KvExtendArgs {
@@ -104,11 +106,12 @@ struct BeamSelectArgs {
   float* out_scores;        // [requests, keep]
   int64_t *out_parent, *out_token;
   unsigned long long* cand;  // workspace [requests * beams, parts, keep]
-  double* stat;              // workspace [requests * beams, parts, 2]
+  double* stat;              // workspace [requests * beams, parts, kBeamWaves, 2]
   int64_t s_request, s_beam;  // elements
   int64_t eos;
   int requests, beams, vocab, keep, parts;
-  int tight;                             // launch_beam_select
+  int tight, type;                       // launch_beam_select
+  double near;
   FastDiv by_beams, by_parts, by_lists;
 };
 

@@ -517,7 +517,7 @@ void check_select(const at::Tensor& logits, const at::Tensor& scores, int64_t ke
   TORCH_CHECK(logits.dim() == 3 && logits.size(1) >= 1 && logits.size(2) >= 1, op,
               ": logits must be [requests, beams, vocabulary], not ", logits.sizes());
   TORCH_CHECK(logits.size(1) * logits.size(2) <= (1ll << 31) - 1, op, ": beams x vocabulary must be below 2^31");
-  TORCH_CHECK(logits.size(1) <= 1024 && logits.size(0) * logits.size(1) <= 65535, op,
+  TORCH_CHECK(logits.size(1) <= kBeamMaxBeams && logits.size(0) * logits.size(1) <= 65535, op,
               ": at most 1,024 beams and 65,535 rows, not ", logits.size(0), " x ", logits.size(1));
   no_grad(logits, op, "logits");
   TORCH_CHECK(scores.scalar_type() == at::kFloat && scores.dim() == 2 && scores.is_contiguous() &&
@@ -566,7 +566,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_hip(const at::Tensor&
   a.parts = beam_select_parts(a.vocab, type);
   const int64_t lists = scores.numel() * a.parts;
   TORCH_CHECK(x.size(1) * a.parts * keep < (1ll << 31), "beam_select: too many beams for this vocabulary");
-  auto work = at::empty({lists * (keep + 2)}, scores.options().dtype(at::kLong));
+  auto work = at::empty({lists * (keep + 2 * kBeamWaves)}, scores.options().dtype(at::kLong));
   a.cand = reinterpret_cast<unsigned long long*>(work.data_ptr<int64_t>());
   a.stat = reinterpret_cast<double*>(a.cand + lists * keep);
   launch_beam_select(a, type, stream_now());

@@ -125,3 +125,116 @@ def test_attention_infinite_values_of_a_split_sequence_gpu(dtype):
     want, bound = _attention(q, kc, vc, table, lens, 0.125)
     out = decode.paged_attention(*(x.cuda() for x in (q, kc, vc, table, torch.tensor(lens, dtype=torch.int32))))
     _close(out, want, bound)
+
+
+# ------------------------------------------------------------------- select
+def _select(logits, scores, keep, finished=None, eos=-1):
+    """(scores, parents, tokens, least gap between different beams that do not tie) in 64 bits,
+    the sums of exponentials exactly rounded."""
+    B, J, V = logits.shape
+    out, gap = [], INF
+    for b in range(B):
+        c = []
+        for j in range(J):
+            s = float(scores[b, j])
+            if finished is not None and bool(finished[b, j]):
+                c.append((-s, j, eos))
+                continue
+            x = logits[b, j].double()
+            m = float(x.max())
+            lse = m + math.log(math.fsum((x - m).exp().tolist()))
+            y = s + (x - lse)
+            some = torch.nonzero(y >= y.topk(min(V, keep)).values[-1])[:, 0]
+            c += [(-float(y[v]), j, int(v)) for v in some]
+        c.sort()
+        gap = min([gap] + [y[0] - x[0] for x, y in zip(c[:keep], c[1:keep + 1]) if x[1] != y[1] and x[0] != y[0]])
+        out.append(c[:keep])
+    return [torch.tensor([[f(r) for r in row] for row in out]) for f in (lambda r: -r[0], lambda r: r[1], lambda r: r[2])] \
+        + [gap]
+
+
+def _selects(device, logits, scores, keep, finished=None, eos=-1):
+    best, parent, token, gap = _select(logits, scores, keep, finished, eos)
+    # two sums of V terms in 64 bits, one after the other at the worst, and the scores' own roundings
+    assert gap > (2 * (logits.shape[2] + 64) + 8 * float(scores.abs().max())) * 2.0 ** -53, gap
+    got = decode.beam_select(logits.to(device), scores.to(device), keep, eos=eos,
+                             finished=None if finished is None else finished.to(device))
+    assert got[1].cpu().tolist() == parent.tolist()
+    assert got[2].cpu().tolist() == token.tolist()
+    # fp32's rounding, and the sums' 2^-24 (5 + 2.25 log V) where no candidates were close
+    err = U * best.abs() + U * (5 + 2.25 * math.log(logits.shape[2]))
+    assert bool(((got[0].cpu().double() - best).abs() <= err).all())
+
+
+@pytest.mark.parametrize("dtype,requests,beams,vocab,keep", [
+    (FP, 2, 8, 50257, 16), (BF, 3, 4, 50262, 8), (HF, 2, 5, 4099, 5), (FP, 4, 3, 1001, 64), (BF, 1, 16, 33, 32),
+    (BF, 33, 8, 16411, 8), (FP, 1, 33, 9001, 40)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_select_equal_rows_go_by_the_lower_beam(device, dtype, requests, beams, vocab, keep):
+    """The same logits at every alignment, with equal scores: each token of the lowest beams first."""
+    x = (3 * torch.randn(requests, 1, vocab, generator=_g(vocab))).to(dtype).expand(-1, beams, -1).contiguous()
+    s = torch.randn(requests, 1, generator=_g(1)).expand(-1, beams).contiguous()
+    _selects(device, x, s, keep)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("device", DEVICES)
+def test_select_beams_closer_than_fp32(device, dtype):
+    """Rows whose log-sum-exps differ by 1e-9 to 1e-6, far below what fp32 holds of them, in
+    an order that is not the beams'; every seventh row twice."""
+    requests, beams, vocab = 4, 8, 20011
+    x = (2 * torch.randn(requests, 1, vocab, generator=_g(4))).to(dtype).expand(-1, beams, -1).contiguous()
+    order = torch.stack([torch.randperm(beams, generator=_g(i)) for i in range(requests)])
+    for b, j in itertools.product(range(requests), range(beams)):
+        # e^-9 of a sum of about e^12: some 1e-9 more a token that comes up from e^-25
+        x[b, j, 100:10100:7] = -25.0
+        x[b, j, 100:100 + 7 * int(order[b, j] // 2) * 3:7] = -9.0 if b < 2 else -5.0
+    s = torch.tensor([0.0, -1.5, 0.25, -30.0])[:, None].expand(-1, beams).contiguous()
+    _selects(device, x, s, 16)
+    _selects(device, x, s, 1)
+    _selects(device, x, s, 64)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_select_close_beams_among_thousands_of_ties(device):
+    """More candidates at the bound than the lists hold, of beams that all but tie."""
+    x = torch.randint(-2, 3, (2, 4, 20011), generator=_g(6)).float()
+    x[:, 1] = x[:, 0]
+    x[:, 1, 7] = -2.0 - 2.0 ** -10  # the upper beam's sum is the smaller one
+    x[:, 0, 7] = -2.0
+    x[1, 3] = x[1, 2]
+    _selects(device, x, torch.zeros(2, 4), 64)
+    _selects(device, x.to(BF), torch.zeros(2, 4), 33)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_select_finished_beams_beside_close_ones(device):
+    """Scores of beams at their end lie exactly on, and an fp32 step beside, those of others."""
+    x = torch.full((3, 4, 4097), -INF)
+    x[:, :, 11] = 0.0  # the one token: log-softmax 0
+    x[:, 3, 12] = -20.0
+    s = torch.tensor([[-1.0, -1.0, -1.0, -1.0], [-1.0, -1.0 - 2.0 ** -23, -1.0, -1.0 + 2.0 ** -24],
+                      [-2.0 ** 20, -2.0 ** 20, -2.0 ** 20 - 0.125, -2.0 ** 20]])
+    f = torch.tensor([[False, True, True, False], [True, False, False, False], [False, False, True, False]])
+    _selects(device, x, s, 4, f, 11)
+    _selects(device, x, s, 2, f, 5)
+
+
+@pytest.mark.gpu
+def test_select_close_beams_captured_gpu():
+    """The second look is the replay's, whatever the first call met."""
+    x = torch.randn(3, 4, 5003, generator=_g(8))
+    s = torch.zeros(3, 4)
+    dx, ds = x.cuda(), s.cuda()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = decode.beam_select(dx, ds, 8)
+    same = x[:, :1].expand(-1, 4, -1).contiguous()
+    for now in (x, same, x, same.flip(0), same):
+        dx.copy_(now)
+        torch.randn(1 << 14, device="cuda").sum().item()
+        graph.replay()
+        best, parent, token, _ = _select(now, s, 8)
+        assert out[1].cpu().tolist() == parent.tolist() and out[2].cpu().tolist() == token.tolist()
+        assert bool(((out[0].cpu().double() - best).abs() <= U * best.abs() + 32 * U).all())
