@@ -95,7 +95,8 @@ def double_heads_loss(model, batch, lm_coef=1.0, mc_coef=1.0):
 def _blocks(tr, x, attend):
     """ln_f output [rows, H] of GPT-2's blocks on the token rows ``x``, without
     dropout; ``attend(layer, qkv [rows, 3H])`` -> [rows, H].  The junction kernels
-    where they cover the model (ops/transformer.py), else torch's."""
+    where they cover the model (ops/transformer.py), else torch's and the model's own
+    activation."""
     eps = float(tr.config.layer_norm_epsilon)
     if _tx.native_ok(tr, x):
         ln = tr.h[0].ln_1
@@ -110,26 +111,35 @@ def _blocks(tr, x, attend):
             ln = tr.h[i + 1].ln_1 if i + 1 < len(tr.h) else tr.ln_f
             h, y = _tx._Impl.resid_ln_fwd(h, p, blk.mlp.c_proj.bias, ln.weight, ln.bias, 0.0, 0, eps, True)[:2]
         return y
+    tanh_gelu = tr.config.activation_function in ("gelu_new", "gelu_pytorch_tanh")
     for i, blk in enumerate(tr.h):
         y = F.layer_norm(x, x.shape[-1:], blk.ln_1.weight, blk.ln_1.bias, eps)
         o = attend(i, torch.addmm(blk.attn.c_attn.bias, y, blk.attn.c_attn.weight))
         x = x + torch.addmm(blk.attn.c_proj.bias, o, blk.attn.c_proj.weight)
         y = F.layer_norm(x, x.shape[-1:], blk.ln_2.weight, blk.ln_2.bias, eps)
-        f = F.gelu(torch.addmm(blk.mlp.c_fc.bias, y, blk.mlp.c_fc.weight), approximate="tanh")
+        f = torch.addmm(blk.mlp.c_fc.bias, y, blk.mlp.c_fc.weight)
+        f = F.gelu(f, approximate="tanh") if tanh_gelu else blk.mlp.act(f)
         x = x + torch.addmm(blk.mlp.c_proj.bias, f, blk.mlp.c_proj.weight)
     return F.layer_norm(x, x.shape[-1:], tr.ln_f.weight, tr.ln_f.bias, eps)
 
 
-def _prompt_attention(qkv, start, lens, longest, nh):
+def _attention_scale(cfg, layer):
+    """What GPT-2's configuration multiplies the scores of a layer (from 0) by."""
+    scale = (cfg.n_embd // cfg.n_head) ** -0.5 if cfg.scale_attn_weights else 1.0
+    return scale / (layer + 1) if cfg.scale_attn_by_inverse_layer_idx else scale
+
+
+def _prompt_attention(qkv, start, lens, longest, nh, scale):
     """Causal attention of packed prompts (host lengths ``lens``), qkv [rows, 3H]."""
     H = qkv.shape[1] // 3
-    if qkv.is_cuda and qkv.dtype == torch.bfloat16 and H // nh == 64 and longest <= _tx.ATTN_MAX_LEN:
+    if (qkv.is_cuda and qkv.dtype == torch.bfloat16 and H // nh == 64 and longest <= _tx.ATTN_MAX_LEN
+            and scale == 0.125):
         n = torch.tensor(lens, dtype=torch.int32, device=qkv.device)
         return _tx._Attention.apply(qkv, start[:-1].contiguous(), n, nh, 0.0, 0, longest)
     out, at = [], 0
     for n in lens:
         q, k, v = (t.view(1, n, nh, H // nh).transpose(1, 2) for t in qkv[at:at + n].split(H, dim=1))
-        o = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        o = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scale)
         out.append(o.transpose(1, 2).reshape(n, H))
         at += n
     return torch.cat(out)
@@ -175,6 +185,7 @@ def generate(model, prompts, *, max_new_tokens=20, num_beams=4, eos=None, token_
     dev, B, J, nh = wte.device, len(prompts), num_beams, cfg.n_head
     H = cfg.n_embd
     hd = H // nh
+    scales = [_attention_scale(cfg, i) for i in range(len(tr.h))]
     longest = max(lens) + max_new_tokens
     pages = sum(-(-n // page_size) for n in lens) + B * J * (1 + -(-max_new_tokens // page_size))
     cache = PagedKV(len(tr.h), nh, hd, B * J, pages, page_size, longest, wte.dtype, dev)
@@ -196,7 +207,7 @@ def generate(model, prompts, *, max_new_tokens=20, num_beams=4, eos=None, token_
     def attend_prompt(layer, qkv):
         k, v = (qkv[:, i * H:(i + 1) * H].view(rows, nh, hd) for i in (1, 2))
         cache.write(layer, k, v, r.slots)
-        return _prompt_attention(qkv, start, lens, max(lens), nh)
+        return _prompt_attention(qkv, start, lens, max(lens), nh, scales[layer])
 
     types = flat(token_types) if token_types is not None else None
     y = _blocks(tr, embed(flat(prompts), r.pos, types), attend_prompt)
@@ -214,7 +225,7 @@ def generate(model, prompts, *, max_new_tokens=20, num_beams=4, eos=None, token_
 
     def attend_token(layer, qkv):
         q, k, v = (qkv[:, i * H:(i + 1) * H].view(B * J, nh, hd) for i in range(3))
-        return cache.attend(layer, q, k, v, max_len=longest).view(B * J, H)
+        return cache.attend(layer, q, k, v, scale=scales[layer], max_len=longest).view(B * J, H)
 
     for t in range(max_new_tokens):
         if t:
