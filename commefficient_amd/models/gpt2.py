@@ -123,6 +123,13 @@ def _blocks(tr, x, attend):
     return F.layer_norm(x, x.shape[-1:], tr.ln_f.weight, tr.ln_f.bias, eps)
 
 
+def can_generate(cfg):
+    """Whether ``generate`` covers models of this configuration: GPT-2 with heads of a
+    width that single-token attention has (ops/decode.py)."""
+    return (getattr(cfg, "model_type", "") == "gpt2" and cfg.n_embd % cfg.n_head == 0
+            and cfg.n_embd // cfg.n_head in (32, 64, 128, 256))
+
+
 def _attention_scale(cfg, layer):
     """What GPT-2's configuration multiplies the scores of a layer (from 0) by."""
     scale = (cfg.n_embd // cfg.n_head) ** -0.5 if cfg.scale_attn_weights else 1.0
@@ -159,6 +166,8 @@ def generate(model, prompts, *, max_new_tokens=20, num_beams=4, eos=None, token_
     training.  The keys and values live in pages (ops/decode.py): a request's
     beams share the prompt's, and no step waits for the GPU (the search ends
     early only where all replies of the batch ended, looked up every 8 tokens).
+    What it does not cover -- other models, heads of other than 32, 64, 128 or 256
+    columns, tokens outside the vocabulary -- is a ValueError before anything runs.
 
     The reference evaluates perplexity and candidate ranking only
     (gpt2_train.py:149-253); replies follow its model and input format."""
@@ -182,9 +191,19 @@ def generate(model, prompts, *, max_new_tokens=20, num_beams=4, eos=None, token_
     wte, wpe = tr.wte.weight, tr.wpe.weight
     if eos is not None and not 0 <= eos < wte.shape[0]:
         raise ValueError("eos %r is not in the vocabulary" % (eos,))
+    for what, lists in (("prompts", prompts), ("token_types", token_types or []),
+                        ("reply_type", [] if reply_type is None else [[reply_type]])):
+        for row in lists:  # (on a GPU the lookup itself would end the process)
+            if not (0 <= min(row) and max(row) < wte.shape[0]):
+                raise ValueError("%s name tokens that are not among the vocabulary's %d" % (what, wte.shape[0]))
     dev, B, J, nh = wte.device, len(prompts), num_beams, cfg.n_head
     H = cfg.n_embd
     hd = H // nh
+    if not can_generate(cfg) or wte.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("generate() covers heads of 32, 64, 128 or 256 columns in bfloat16, float16 or float32, "
+                         "not %d heads over %d columns in %s" % (nh, H, wte.dtype))
+    if page_size < 1:
+        raise ValueError("a page holds at least a token, not %r" % (page_size,))
     scales = [_attention_scale(cfg, i) for i in range(len(tr.h))]
     longest = max(lens) + max_new_tokens
     pages = sum(-(-n // page_size) for n in lens) + B * J * (1 + -(-max_new_tokens // page_size))

@@ -293,3 +293,20 @@ def test_generate_follows_the_configuration_bf16_gpu(cfg):
             x = ref.lm_head(ref.transformer(torch.tensor([p + tokens], device="cuda"))[0][0])
         lp = torch.log_softmax(x.double(), 1)[len(p) - 1:-1]
         assert abs(float(lp.gather(1, torch.tensor(tokens, device="cuda")[:, None]).mean()) - score) < 0.25
+
+
+def test_generate_refuses_before_it_runs(monkeypatch):
+    """Tokens outside the vocabulary, heads that single-token attention does not have and other
+    types are refused on the host, with nothing run."""
+    from commefficient_amd.models import gpt2
+    m = _gpt2(FP, "cpu")
+    monkeypatch.setattr(gpt2, "PagedKV", None)  # (what a run begins with)
+    ok = dict(prompts=[[1, 2], [3]], token_types=[[4, 5], [6]], reply_type=7)
+    for bad in (dict(prompts=[[1, 997], [3]]), dict(prompts=[[1, 2], [-1]]), dict(token_types=[[4, 5], [997]]),
+                dict(token_types=[[4, -2], [5]]), dict(reply_type=997), dict(reply_type=-1), dict(page_size=0),
+                dict(page_size=-4), dict(eos=-1)):
+        with pytest.raises(ValueError):
+            gpt2.generate(m, **{**ok, **bad})
+    for other in (_gpt2(FP, "cpu", n_embd=96, n_head=2), _gpt2(FP, "cpu", n_head=4), m.double()):
+        with pytest.raises(ValueError, match="columns"):
+            gpt2.generate(other, **ok)
