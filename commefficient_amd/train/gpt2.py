@@ -21,7 +21,7 @@ import torch
 
 from ..data.fed_persona import SPECIAL_TOKENS, FedPERSONA, SyntheticPersona
 from ..data.persona_loader import PersonaFedLoader, PersonaValLoader
-from ..models.gpt2 import ATTR_TO_SPECIAL_TOKEN, GPT2DoubleHeads
+from ..models.gpt2 import ATTR_TO_SPECIAL_TOKEN, GPT2DoubleHeads, can_generate
 from ..parallel import dist
 from ..parallel.fed_model import FedModel
 from ..parallel.server import FedOptimizer
@@ -167,8 +167,10 @@ def main(args):
     # OpenAI-GPT, gpt2_train.py:262-267 -- not the checkpoint itself)
     family = "gpt2" if "gpt2" in args.model_checkpoint else "openai-gpt"
     model = GPT2DoubleHeads(args.model_checkpoint if not args.do_test else family, **dims)
-    if args.replies and getattr(model.model.config, "model_type", "") != "gpt2":
-        raise ValueError("--replies covers GPT-2 models")
+    cfg = model.model.config
+    if args.replies and not (can_generate(cfg) and args.max_reply < cfg.n_positions):
+        raise ValueError("--replies covers GPT-2 models with heads of 32, 64, 128 or 256 columns and replies "
+                         "shorter than their positions")
     if tokenizer is not None:
         model.model.resize_token_embeddings(len(tokenizer))
     args.len_tokenizer = model.model.config.vocab_size
@@ -230,9 +232,6 @@ def main(args):
             progress["epoch"], progress["iter"] = epoch + 1, 0
         if args.max_rounds and fed.round_idx >= args.max_rounds:
             break
-    if args.replies and ctx.is_main:
-        for r in sample_replies(fed, test_loader, args, tokenizer):
-            print(r)
     profiler.close(fed.timer)
     train_loader.close()  # the record worker processes, if any
     fed.finalize()
@@ -240,4 +239,7 @@ def main(args):
         save_checkpoint(fed, args, progress)
     if writer is not None:
         writer.close()
+    if args.replies and ctx.is_main:  # (with the run's results safe, and no rank waiting)
+        for r in sample_replies(fed, test_loader, args, tokenizer):
+            print(r)
     return fed

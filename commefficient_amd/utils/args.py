@@ -271,6 +271,11 @@ def validate_args(args) -> None:
                 "on the server (fed_worker.py:227-228); use --virtual_momentum")
         if args.error_type == "local":
             bad("--mode sketch requires --error_type none or virtual (fed_worker.py:221-222)")
+    replies = getattr(args, "replies", 0)
+    if replies < 0:
+        bad("--replies is a number of dialogues")
+    if replies and not (1 <= args.num_beams <= 32 and args.max_reply >= 1):
+        bad("--replies needs 1 to 32 --num_beams and a --max_reply of at least one token")
     if args.mode == "true_topk" and args.error_type != "virtual":
         bad("--mode true_topk requires --error_type virtual (fed_aggregator.py:512)")
     if args.mode == "local_topk" and args.error_type not in ("local", "none"):

@@ -310,3 +310,42 @@ def test_generate_refuses_before_it_runs(monkeypatch):
     for other in (_gpt2(FP, "cpu", n_embd=96, n_head=2), _gpt2(FP, "cpu", n_head=4), m.double()):
         with pytest.raises(ValueError, match="columns"):
             gpt2.generate(other, **ok)
+
+
+# ------------------------------------------------------------------- driver
+def _driver_args(tmp_path, monkeypatch, *extra):
+    from commefficient_amd.utils.args import parse_args
+    monkeypatch.chdir(tmp_path)
+    return parse_args(default_lr=4e-2, argv=[
+        "--dataset_name", "PERSONA", "--model", "GPT2DoubleHeads", "--synthetic", "--num_clients", "6", "--num_workers",
+        "2", "--local_batch_size", "2", "--mode", "uncompressed", "--local_momentum", "0", "--num_epochs", "1",
+        "--max_rounds", "1", "--valid_batch_size", "2", "--num_candidates", "2", "--gpt2_size", "tiny", "--device",
+        "cpu", "--replies", "2", *extra], probe_port=False)
+
+
+def test_replies_come_after_the_checkpoint(tmp_path, monkeypatch):
+    """A reply that fails costs neither the checkpoint nor the server's state."""
+    from commefficient_amd.train import gpt2 as driver
+    args = _driver_args(tmp_path, monkeypatch, "--checkpoint", "--checkpoint_path", str(tmp_path / "ck"))
+
+    def fails(*a):
+        raise RuntimeError("no reply")
+    monkeypatch.setattr(driver, "sample_replies", fails)
+    with pytest.raises(RuntimeError, match="no reply"):
+        driver.main(args)
+    saved = sorted(p.name for p in tmp_path.glob("ck*"))
+    assert saved == ["ckGPT2DoubleHeads.fedstate.pt", "ckGPT2DoubleHeads.pt"]
+
+
+@pytest.mark.parametrize("extra", [["--num_beams", "33"], ["--num_beams", "0"], ["--max_reply", "0"], ["--replies", "-1"]],
+                         ids=" ".join)
+def test_reply_arguments_are_checked_when_parsed(extra, tmp_path, monkeypatch):
+    with pytest.raises(ValueError, match="--replies"):
+        _driver_args(tmp_path, monkeypatch, *extra)
+
+
+def test_replies_longer_than_the_model_are_refused_before_training(tmp_path, monkeypatch):
+    from commefficient_amd.train import gpt2 as driver
+    monkeypatch.setattr(driver, "FedModel", None)  # (what training begins with)
+    with pytest.raises(ValueError, match="--replies"):
+        driver.main(_driver_args(tmp_path, monkeypatch, "--max_reply", "1024"))
