@@ -62,20 +62,40 @@ void no_grad(const at::Tensor& t, const char* op, const char* name) {
               " requires a gradient, and this operator has none: call it under torch.no_grad()");
 }
 
-// [pages, kv heads, page, dim], any strides but a unit one over dim, every
-// element an address of its own
-void check_cache(const at::Tensor& c, const char* op, const char* name) {
+// Whether every element has an address of its own (up to 6 dimensions): each dimension's
+// steps are longer than all that the dimensions of shorter ones span.
+bool own_addresses(const at::Tensor& t) {
+  std::pair<int64_t, int64_t> dims[6];  // (stride, size), the shortest strides first
+  int n = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) <= 1) continue;
+    int at = n++;
+    for (; at > 0 && dims[at - 1].first > t.stride(d); --at) dims[at] = dims[at - 1];
+    dims[at] = {t.stride(d), t.size(d)};
+  }
+  int64_t span = 0;  // the furthest element so far
+  for (int i = 0; i < n; ++i) {
+    if (dims[i].first <= span) return false;
+    span += dims[i].first * (dims[i].second - 1);
+  }
+  return true;
+}
+
+// [pages, kv heads, page, dim], any strides but a unit one over dim; a cache that is
+// written has an address for every element
+void check_cache(const at::Tensor& c, bool written, const char* op, const char* name) {
   TORCH_CHECK(c.dim() == 4 && c.size(1) >= 1 && c.size(2) >= 1 && c.size(3) >= 1, op, ": ", name,
               " must be [pages, kv heads, page size, head dim], not ", c.sizes());
   TORCH_CHECK(c.size(3) == 1 || c.stride(3) == 1, op, ": ", name, " needs a unit stride over the head's columns");
-  TORCH_CHECK(c.is_non_overlapping_and_dense() || c.numel() == 0 ||
-                  (c.stride(0) > 0 && c.stride(1) > 0 && c.stride(2) > 0),
-              op, ": ", name, " is an expanded view");
+  for (int d = 0; d < 3; ++d)
+    TORCH_CHECK(c.size(d) <= 1 || c.numel() == 0 || c.stride(d) > 0, op, ": ", name, " is an expanded view");
+  TORCH_CHECK(!written || c.numel() == 0 || own_addresses(c), op, ": ", name, " overlaps itself: strides ", c.strides(),
+              " of ", c.sizes());
 }
 
-void check_pair(const at::Tensor& kc, const at::Tensor& vc, const char* op) {
-  check_cache(kc, op, "the key cache");
-  check_cache(vc, op, "the value cache");
+void check_pair(const at::Tensor& kc, const at::Tensor& vc, bool written, const char* op) {
+  check_cache(kc, written, op, "the key cache");
+  check_cache(vc, written, op, "the value cache");
   TORCH_CHECK(kc.sizes() == vc.sizes() && kc.scalar_type() == vc.scalar_type(), op,
               ": key and value cache differ: ", kc.scalar_type(), " ", kc.sizes(), " and ", vc.scalar_type(), " ",
               vc.sizes());
@@ -235,7 +255,7 @@ void check_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc,
                  const at::Tensor& slots) {
   const char* op = "kv_write";
   decode_type(kc, op, "the key cache");
-  check_pair(kc, vc, op);
+  check_pair(kc, vc, true, op);
   check_page(kc.size(2), 0, op);
   TORCH_CHECK(kc.size(0) * kc.size(2) < (1ll << 31), op, ": the caches must hold less than 2^31 slots, not ",
               kc.size(0), " pages of ", kc.size(2));
@@ -306,6 +326,8 @@ void check_reorder(const at::Tensor& parent, const at::Tensor& table, const at::
               kv.sizes());
   for (int d = 0; d < 5; ++d)
     TORCH_CHECK(kv.size(d) <= 1 || kv.stride(d) > 0, op, ": kv is an expanded view");
+  TORCH_CHECK(kv.numel() == 0 || own_addresses(kv), op, ": kv overlaps itself: strides ", kv.strides(), " of ",
+              kv.sizes());
   same_device(kv, table, op, "kv");
   check_page(kv.size(4), table.size(1), op);
   TORCH_CHECK(2 * kv.size(0) * kv.size(3) * kv.size(4) * kv.size(5) < (1ll << 31), op,
@@ -368,7 +390,7 @@ void check_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
                      const at::Tensor& lens, const OptTensor& k, const OptTensor& v) {
   const char* op = "paged_attention";
   decode_type(kc, op, "the key cache");
-  check_pair(kc, vc, op);
+  check_pair(kc, vc, given(k), op);
   const int64_t hd = kc.size(3);
   TORCH_CHECK(hd == 32 || hd == 64 || hd == 128 || hd == 256, op, ": head dim 32, 64, 128 or 256, not ", hd);
   TORCH_CHECK(q.dim() == 3 && q.scalar_type() == kc.scalar_type() && q.size(2) == hd && q.size(1) >= 1 &&

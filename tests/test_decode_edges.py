@@ -349,3 +349,39 @@ def test_replies_longer_than_the_model_are_refused_before_training(tmp_path, mon
     monkeypatch.setattr(driver, "FedModel", None)  # (what training begins with)
     with pytest.raises(ValueError, match="--replies"):
         driver.main(_driver_args(tmp_path, monkeypatch, "--max_reply", "1024"))
+
+
+# ----------------------------------------------------------------- refusals
+def test_caches_that_overlap_themselves_are_not_written():
+    """Slots that share memory would be racing stores: refused where a call writes, whatever the
+    strides' order; caches with gaps, in any order of their dimensions, are not."""
+    z, i = torch.zeros, lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    rows = dict(k=z(3, 2, 32), v=z(3, 2, 32))
+    one = dict(q=z(3, 2, 32), table=i(3, 1), lens=i(3))
+    buf = torch.zeros(1 << 16)
+    bad = [(1, 1, 1, 1), (512, 256, 16, 1), (256, 512, 32, 1), (2048, 31, 64, 1), (32, 1024, 96, 1)]
+    good = [(512, 256, 32, 1), (512, 32, 64, 1), (40, 160, 320, 1), (2048, 1024, 96, 1), (32, 4096, 512, 1)]
+    for strides in bad + good:
+        kc, vc = (buf.as_strided((4, 2, 8, 32), strides, at) for at in (0, 1 << 15))
+        calls = [lambda: decode.kv_write(**rows, k_cache=kc, v_cache=vc, slots=torch.arange(3)),
+                 lambda: decode.paged_attention(k_cache=kc, v_cache=vc, **one, **rows)]
+        for call in calls:
+            if strides in bad:
+                with pytest.raises(RuntimeError, match="overlaps itself"):
+                    call()
+            else:
+                call()
+        decode.paged_attention(k_cache=kc, v_cache=vc, **one)  # (reads only)
+    six = dict(parent=torch.zeros(1, 2, dtype=torch.int64), table=i(2, 2), lens=i(2))
+    decode.beam_reorder(**six, kv=buf.as_strided((2, 2, 4, 1, 8, 32), (4096, 2048, 512, 7, 40, 1)))
+    for strides in ((2048, 1024, 250, 1, 32, 1), (100, 1024, 256, 1, 32, 1), (2048, 1024, 256, 1, 31, 1)):
+        with pytest.raises(RuntimeError, match="beam_reorder.*overlaps itself"):
+            decode.beam_reorder(**six, kv=buf.as_strided((2, 2, 4, 1, 8, 32), strides))
+
+
+def test_caches_of_one_head_or_page_take_any_stride_there():
+    """A dimension of one element has no step to be wrong."""
+    kc, vc = (torch.randn(1 << 12, generator=_g(j)).as_strided((6, 1, 8, 32), (300, 0, 32, 1)) for j in (1, 2))
+    k = torch.randn(3, 1, 32)
+    decode.kv_write(k, k, kc, vc, torch.tensor([0, 47, 9]))
+    assert torch.equal(kc[5, :, 7], k[1]) and torch.equal(vc[1, :, 1], k[2])
