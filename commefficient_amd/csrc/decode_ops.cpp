@@ -538,7 +538,8 @@ void check_select(const at::Tensor& logits, const at::Tensor& scores, int64_t ke
   decode_type(logits, op, "logits");
   TORCH_CHECK(logits.dim() == 3 && logits.size(1) >= 1 && logits.size(2) >= 1, op,
               ": logits must be [requests, beams, vocabulary], not ", logits.sizes());
-  TORCH_CHECK(logits.size(1) * logits.size(2) <= (1ll << 31) - 1, op, ": beams x vocabulary must be below 2^31");
+  TORCH_CHECK(logits.size(1) * logits.size(2) <= (1ll << 31) - (1 << 16), op,
+              ": beams x vocabulary must be at most 2^31 - 2^16, not ", logits.size(1), " x ", logits.size(2));
   TORCH_CHECK(logits.size(1) <= kBeamMaxBeams && logits.size(0) * logits.size(1) <= 65535, op,
               ": at most 1,024 beams and 65,535 rows, not ", logits.size(0), " x ", logits.size(1));
   no_grad(logits, op, "logits");

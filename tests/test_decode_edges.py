@@ -385,3 +385,12 @@ def test_caches_of_one_head_or_page_take_any_stride_there():
     k = torch.randn(3, 1, 32)
     decode.kv_write(k, k, kc, vc, torch.tensor([0, 47, 9]))
     assert torch.equal(kc[5, :, 7], k[1]) and torch.equal(vc[1, :, 1], k[2])
+
+
+def test_select_refuses_rows_whose_places_would_pass_32_bits():
+    """The kernels count a row's elements in 32 bits, with room for a workgroup behind its end."""
+    most = 2 ** 31 - 2 ** 16
+    for beams, vocab in ((1, most + 1), (1, 2 ** 31 - 1), (2, 2 ** 30)):
+        with pytest.raises(RuntimeError, match="beams x vocabulary"):
+            decode.beam_select(torch.zeros(1, 1, 1)[:0].expand(0, beams, vocab), torch.zeros(0, beams))
+    assert decode.beam_select(torch.zeros(1, 1, 1)[:0].expand(0, 1, most), torch.zeros(0, 1))[0].shape == (0, 1)
