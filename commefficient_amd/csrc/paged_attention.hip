@@ -677,6 +677,8 @@ void plan_paged_attention(PagedAttnArgs& a, DecodeType t, int64_t longest) {
   const int64_t groups = static_cast<int64_t>(a.n) * a.kv_heads * ((group + 15) / 16);
   const int64_t tiles = (longest + kTile - 1) / kTile;
   a.waves = tiles <= 2 || (tiles <= 4 && groups >= 2048) ? 1 : tiles > 8 && a.dim * (t == kF32 ? 4 : 2) <= 256 ? 8 : 4;
+  // (a launch has less than 2^32 threads; sequences x heads are at most 2^24)
+  while (groups * a.waves * 64 >= 1ll << 32) a.waves = a.waves == 8 ? 4 : 1;
   int64_t split = 1;
   if (groups > 0 && tiles >= 6 * a.waves) split = (1024 + groups - 1) / groups;
   const int64_t most = tiles / (2 * a.waves);

@@ -394,3 +394,21 @@ def test_select_refuses_rows_whose_places_would_pass_32_bits():
         with pytest.raises(RuntimeError, match="beams x vocabulary"):
             decode.beam_select(torch.zeros(1, 1, 1)[:0].expand(0, beams, vocab), torch.zeros(0, beams))
     assert decode.beam_select(torch.zeros(1, 1, 1)[:0].expand(0, 1, most), torch.zeros(0, 1))[0].shape == (0, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_of_millions_of_rows_gpu(dtype):
+    """2^23 sequences whose tables allow 320 tokens: 8 waves each would pass a launch's 2^32 threads."""
+    n, page = 1 << 23, 320
+    g = _g(2)
+    kc, vc = (torch.randn(5, 1, page, 32, generator=g).to(dtype).cuda() for _ in range(2))
+    q = torch.randn(1, 1, 32, generator=g).to(dtype)
+    table = torch.arange(5).int().repeat(-(-n // 5))[:n].view(n, 1)
+    lens = torch.zeros(n, dtype=torch.int32)
+    some = [0, 1, 12345, n // 2, n - 1]
+    lens[some] = torch.tensor([320, 1, 77, 129, 300], dtype=torch.int32)
+    out = decode.paged_attention(q.cuda().expand(n, 1, 32), kc, vc, table.cuda(), lens.cuda())
+    assert int((out != 0).any(2).sum()) == len(some)
+    want, bound = _attention(q.expand(len(some), 1, 32), kc.cpu(), vc.cpu(), table[some], lens[some].tolist(), 32 ** -0.5)
+    _close(out[some], want, bound)
