@@ -45,6 +45,8 @@ def _attention(q, kc, vc, table, lens, scale):
     out, bound = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
     pieces = {BF: 2.0 ** -16, HF: 2.0 ** -22, FP: 0.0}[q.dtype]
     for i, n in enumerate(lens):
+        if n == 0:
+            continue
         ids = table[i, :-(-n // page)].long()
         k, v = (c[ids].transpose(1, 2).reshape(-1, kh, dim)[:n].double() for c in (kc, vc))
         for h in range(heads):
@@ -412,3 +414,31 @@ def test_attention_of_millions_of_rows_gpu(dtype):
     assert int((out != 0).any(2).sum()) == len(some)
     want, bound = _attention(q.expand(len(some), 1, 32), kc.cpu(), vc.cpu(), table[some], lens[some].tolist(), 32 ** -0.5)
     _close(out[some], want, bound)
+
+
+@pytest.mark.parametrize("append", [False, True])
+@pytest.mark.parametrize("lens", [[1, 33, 64, 17, 0], [65, 1, 256, 200, 97], [257, 600, 12, 333, 480], [5000, 3077]],
+                         ids=["1wave", "4waves", "8waves", "split"])
+@pytest.mark.parametrize("kv_heads,group,dim,page", [(2, 2, 32, 16), (1, 2, 64, 1), (2, 2, 128, 24), (2, 1, 128, 16),
+                                                     (1, 1, 32, 5), (1, 1, 256, 8), (1, 4, 256, 16)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_fp32_variants(device, kv_heads, group, dim, page, lens, append):
+    """Every form that fp32 caches take: groups of one and two heads on the vector units, others on
+    the matrix units, each with 1, 4 and 8 waves and split."""
+    q, kc, vc, table = _cache(FP, lens, kv_heads, group, dim, page, seed=dim + group)
+    want, bound = _attention(q, kc, vc, table, lens, dim ** -0.5)
+    kw = {}
+    if append:  # the last rows come with the call, the slots hold junk
+        last = [(table[i, (n - 1) // page].long(), (n - 1) % page) for i, n in enumerate(lens) if n]
+        k, v = (torch.zeros(len(lens), kv_heads, dim) for _ in range(2))
+        wk, wv = kc.clone(), vc.clone()
+        for i, (p, o) in zip([i for i, n in enumerate(lens) if n], last):
+            k[i], v[i] = kc[p, :, o], vc[p, :, o]
+            kc[p, :, o], vc[p, :, o] = NAN, INF
+        kw = dict(k=k.to(device), v=v.to(device))
+    dk, dv = kc.to(device), vc.to(device)
+    out = decode.paged_attention(q.to(device), dk, dv, table.to(device),
+                                 torch.tensor(lens, dtype=torch.int32, device=device), **kw)
+    _close(out, want, bound)
+    if append:
+        assert torch.equal(dk.cpu(), wk) and torch.equal(dv.cpu(), wv)
