@@ -274,11 +274,12 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamSelectArgs a) {
   }
 }
 
-// exp(x), -701 <= x <= 0: 2^n e^r with n next to x / log 2 (the low bits of a sum that holds
+// exp(x), x <= 0, from -700 on e^-700: 2^n e^r with n next to x / log 2 (the low bits of a sum that holds
 // no fraction), |r| < 0.35 and e^r its series to 4e-18; off by some 1e-15
 __device__ __forceinline__ double exp64(double x) {
   constexpr double kLog2 = 0.69314718055994530942, kHi = 0x1.62e42fefap-1;  // (the upper part of log(2))
   constexpr double kWhole = 0x1.8p52;
+  x = fmax(x, -700.0);
   constexpr double kTerm[14] = {1.0, 1.0, 0.5, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
                                 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600, 1.0 / 6227020800.0};
   const double sum = fma(x, 1.0 / kLog2, kWhole), n = sum - kWhole;
@@ -297,7 +298,6 @@ __device__ __forceinline__ double row_sum(const BeamSelectArgs& a, int64_t at, d
   constexpr int EB = T == kF32 ? 4 : 2, GE = 16 / EB, kAhead = 8;
   const unsigned char* p = static_cast<const unsigned char*>(a.logits) + at * EB;
   const int full = a.vocab / GE, tid = threadIdx.x;
-  const float least = static_cast<float>(m) - 700.f;  // (-inf: e^-700 of the greatest term)
   auto load = [&](int i) {
     v4u u = {kLow<T>, kLow<T>, kLow<T>, kLow<T>};
     if (i < full) __builtin_memcpy(&u, p + static_cast<int64_t>(i) * 16, 16);
@@ -314,13 +314,13 @@ __device__ __forceinline__ double row_sum(const BeamSelectArgs& a, int64_t at, d
     u[kAhead - 1] = load(i + kAhead * kThreads);
 #pragma unroll
     for (int e = 0; e < GE; ++e)
-      sum += exp64(fmaxf(to_float<T>(EB == 4 ? now[e % 4] : (now[e / 2] >> (16 * (e & 1))) & 0xffffu), least) - m);
+      sum += exp64(to_float<T>(EB == 4 ? now[e % 4] : (now[e / 2] >> (16 * (e & 1))) & 0xffffu) - m);
   }
   const int v = full * GE + tid;
   if (v < a.vocab) {
     uint32_t x = 0;
     __builtin_memcpy(&x, p + static_cast<int64_t>(v) * EB, EB);
-    sum += exp64(fmaxf(to_float<T>(x), least) - m);
+    sum += exp64(to_float<T>(x) - m);
   }
   return sum;
 }

@@ -197,6 +197,16 @@ def test_select_beams_closer_than_fp32(device, dtype):
     _selects(device, x, s, 64)
 
 
+@pytest.mark.parametrize("scale", [1e-6, 1e5, 1e12, 1e37])
+@pytest.mark.parametrize("device", DEVICES)
+def test_select_equal_rows_of_any_size(device, scale):
+    """Tiny and huge logits, whose sums are those of one term or of all alike."""
+    x = (scale * torch.rand(2, 1, 3001, generator=_g(12))).expand(-1, 6, -1).contiguous()
+    x[1, 2:4] = x[1, 4:6].flip(1)  # (other rows with the same sum, but for its order)
+    x[1, 2:4, 77] = x[1, :1].amax() + 2 * scale
+    _selects(device, x, torch.zeros(2, 6), 12)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_select_close_beams_among_thousands_of_ties(device):
     """More candidates at the bound than the lists hold, of beams that all but tie."""
