@@ -32,7 +32,9 @@
 // maxima, so nothing below that (the largest such of the waves) can be among
 // the `keep` best.  It is found by bits with a ballot a bit, some 2 keep to 4
 // keep elements pass, and those are ranked by counting.  Where more than the
-// lists hold pass (thousands of equal logits) `keep` rounds of an argmax take over.
+// lists hold pass (thousands of equal logits; `keep` near 64, where the bound is the
+// least of a wave's lanes) `keep` rounds of an argmax take over: 16 rows of 50,262
+// logits 450 us for 64 places.
 #include <hip/hip_runtime.h>
 #include <cfloat>
 #include <cmath>
@@ -411,45 +413,63 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(BeamSelectArgs a) {
   }
   for (int c = tid + kHeld * kThreads; c < all; c += kThreads)
     most = max(most, static_cast<uint32_t>(score(c, fetch(c)).value >> 32));
-  uint32_t bound = 0;
-  if (a.keep <= 32 || all > kHeld * kThreads) {
-    bound = wave_bound(most, a.keep);
-    if (lane == 0) s_u[0][w] = bound;
-    __syncthreads();
-    bound = max(max(s_u[0][0], s_u[0][1]), max(s_u[0][2], s_u[0][3]));
-  } else {
-    // many places: the keep-th largest of all candidates, so that few more than
-    // those are left to rank (16 beams, 64 places: 13.0 against
-    // 150 us; for up to 32 the search costs what it saves)
+  // the upper half of the keep-th largest of all candidates (or less by bits that do not
+  // matter), by bits
+  auto counted = [&] {
+    uint32_t bound = 0;
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t c = bound | 1u << bit;
       int n = 0;
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) n += __popcll(__ballot(static_cast<uint32_t>(mine[i].value >> 32) >= c));
+      for (int i = kHeld * kThreads; i < all; i += kThreads)
+        n += __popcll(__ballot(i + tid < all && static_cast<uint32_t>(score(i + tid, fetch(i + tid)).value >> 32) >= c));
       if (lane == 0) s_u[bit & 1][w] = n;
       __syncthreads();  // (the other half is read until the next one)
       n = s_u[bit & 1][0] + s_u[bit & 1][1] + s_u[bit & 1][2] + s_u[bit & 1][3];
       if (n >= a.keep) bound = c;
       if (n == a.keep) break;
     }
-  }
-  // (down to what may belong above it; up to 0x000fffff no number's upper half)
-  if (bound > 0x000fffffu) {
-    const double x = unordered(static_cast<u64>(bound) << 32);
-    bound = static_cast<uint32_t>(ordered(x - near - 0x1p-50 * fabs(x)) >> 32);
-  }
-  bound = max(bound, 1u);
-  auto pass = [&](const Best& x) {
+    return bound;
+  };
+  int n = 0;
+  auto pass = [&](const Best& x, uint32_t bound) {
     if (static_cast<uint32_t>(x.value >> 32) >= bound) {
       const int at = atomicAdd(&s_n, 1);  // (any order: the list is ranked)
       if (at < kJoinList) s_list[at] = x;
     }
   };
+  auto make_list = [&](uint32_t bound) {
+    // (down to what may belong above it; up to 0x000fffff no number's upper half)
+    if (bound > 0x000fffffu) {
+      const double x = unordered(static_cast<u64>(bound) << 32);
+      bound = static_cast<uint32_t>(ordered(x - near - 0x1p-50 * fabs(x)) >> 32);
+    }
+    bound = max(bound, 1u);
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) pass(mine[i]);
-  for (int c = tid + kHeld * kThreads; c < all; c += kThreads) pass(score(c, fetch(c)));
-  __syncthreads();
-  const int n = s_n;
+    for (int i = 0; i < kHeld; ++i) pass(mine[i], bound);
+    for (int c = tid + kHeld * kThreads; c < all; c += kThreads) pass(score(c, fetch(c)), bound);
+    __syncthreads();
+    n = s_n;
+  };
+  const bool held_all = all <= kHeld * kThreads;
+  if (a.keep <= 32 || !held_all) {
+    const uint32_t bound = wave_bound(most, a.keep);
+    if (lane == 0) s_u[0][w] = bound;
+    __syncthreads();
+    make_list(max(max(s_u[0][0], s_u[0][1]), max(s_u[0][2], s_u[0][3])));
+  } else {
+    // many places: counted, so that few more than those are left to rank (8 requests of 16
+    // beams, 64 places: 16 against 131 us; for up to 32 the search costs what it saves)
+    make_list(counted());
+  }
+  if (n > kJoinList && !held_all) {
+    // .. and where the list does not hold what the waves' bound lets pass (16 beams of
+    // 50,262, 64 places: 92 against 400 us)
+    __syncthreads();
+    if (tid == 0) s_n = 0;
+    make_list(counted());  // (barriers in it)
+  }
   auto rank_list = [&] {
     for (int c = tid >> 2; c < n; c += kThreads / 4) {
       const Best x = s_list[c];
@@ -545,8 +565,8 @@ int beam_select_parts(int vocab, DecodeType t) {
 void launch_beam_select(BeamSelectArgs a, DecodeType t, hipStream_t stream) {
   if (a.requests == 0) return;
   // a tighter bound costs a search more and saves passing elements: worth it
-  // where throughput counts (64 x 8 beams 24.6 against 26.6 us), not for few
-  // workgroups (1 x 4 beams 11.6 against 11.1); its table holds 16 of a wave
+  // where throughput counts (64 x 8 beams 25.9 against 28.5 us), not for few
+  // workgroups (1 x 4 beams 11.7 against 11.6); its table holds 16 of a wave
   a.tight = a.keep <= 16 && static_cast<int64_t>(a.requests) * a.beams * a.parts >= 512;
   a.type = t;
   a.near = 2.0 * 0x1p-24 * (5.0 + 2.25 * std::log(static_cast<double>(a.vocab)));
