@@ -119,8 +119,8 @@ __device__ __forceinline__ Best block_best(Best x, Best* lds) {
 
 // 64 x 8 rows of 50,262 bf16 logits, a quarter of them at their end: 18 us for
 // 39 MB, bound by the chain of its phases (loads, maxima, search, exponentials,
-// list, ranks): some 800 vector instructions a wave, a sixth of its life, and
-// neither fewer of them nor more waves a SIMD shorten it; four rows 7 us.
+// list, ranks), which all parts walk at about the same time: nearly the whole grid
+// is resident at once; four rows 7 us.
 // Part `blockIdx.x` of row `blockIdx.y`: every wave's (maximum, sum of exponentials
 // beside it) into stat, the best `keep` as ordered(logit) << 32 | ~index into cand, in
 // their order, 0 where there are fewer

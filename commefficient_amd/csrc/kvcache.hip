@@ -21,8 +21,10 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 // launch, two scans and the chain row -> sequence -> page.  So one workgroup
 // does all of it with the sequences' plan in LDS; only batches too large for
 // that (kFused) leave the rows to a second launch over the whole chip.  16
-// prompts of up to 500 tokens 7.1 us (an empty launch 1.4, the scans 2.8, the
-// rows 2.9), one token for 4,096 sequences 11.1.
+// prompts of up to 500 tokens 7.5 us (an empty launch 1.4, the scans 2.8, the
+// rows 2.9), one token for 4,096 sequences 11.1.  Against the two launches:
+// 1,024 sequences 7.9 to 10.0 us, 4,096 11.2 to 15.0, 8,192 19.3 to 21.6; 1,000
+// with 8 rows each 11.5 either way.
 constexpr int kScan = 1024, kEach = 4;  // threads of the scan, sequences a thread takes at once
 constexpr int kFused = 8192;            // sequences and rows of a single launch
 

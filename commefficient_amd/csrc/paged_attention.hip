@@ -29,8 +29,8 @@
 // powers of two), which a wave votes on: the cross-lane maximum and the rescaling
 // of O run a few times a sequence, not once a tile.
 // Reached: 8 sequences of up to 65,536 tokens, 32 heads over 8 of 128, bf16:
-// 1.21 GB at 5.0 TB/s; 128 x 8 heads of 128, up to 1,024 tokens: 271 MB at 4.6;
-// 64 x 12 of 64: 103 MB in 27 us, 7 of them start and end; one short reply 6.
+// 1.21 GB at 4.9 to 5.0 TB/s; 128 x 8 heads of 128, up to 1,024 tokens: 271 MB at 4.6;
+// 64 x 12 of 64: 103 MB in 27 us (a copy of as much 21); one short reply 6.5.
 #include <hip/hip_runtime.h>
 #include <cfloat>
 #include <cstdint>
@@ -635,7 +635,9 @@ template <DecodeType T, int HD, int W>
 void launch_group(const PagedAttnArgs& a, hipStream_t stream) {
   if constexpr (T == kF32) {
     if (a.group == 1) return launch_one<T, HD, W, 1>(a, stream);
-    if constexpr (HD <= 128) {  // (a second head of 256 columns does not fit the registers)
+    // (256 columns: the registers of two waves a SIMD leave 20 bytes a lane of one head in
+    // scratch, more of a second one, and 124 to 128 of the MFMA form)
+    if constexpr (HD <= 128) {
       if (a.group == 2) return launch_one<T, HD, W, 2>(a, stream);
     }
   }

@@ -15,9 +15,10 @@ a length:
 
 HIP kernels in csrc/kvcache.hip, paged_attention.hip and beam.hip, plain loops
 for CPU tensors in csrc/decode_ops.cpp; both check their arguments alike (but for
-the alignment that a kernel needs) and raise RuntimeError.  The operators run on the current stream of their tensors'
-device, allocate their outputs and workspaces per call and read nothing back,
-so a step can be captured into a graph.  None of them has a gradient.
+the alignment that a kernel needs) and raise RuntimeError.  The operators run on
+the current stream of their tensors' device, allocate their outputs and workspaces
+per call and read nothing back, so a step can be captured into a graph.  None of
+them has a gradient.
 """
 from __future__ import annotations
 
@@ -64,8 +65,9 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
              slots: torch.Tensor) -> None:
     """Rows k, v [rows, kv heads, head dim] into their slots (int64 [rows]) of one
     layer's caches [pages, kv heads, page size, head dim]; any row, head, page and
-    slot strides that leave the caches' elements addresses of their own.  Slots outside the cache (-1) are skipped.  The slots of one
-    call are distinct: a slot named twice ends with a mixture of its rows."""
+    slot strides that leave the caches' elements addresses of their own.  Slots
+    outside the cache (-1) are skipped.  The slots of one call are distinct: a slot
+    named twice ends with a mixture of its rows."""
     _ops().kv_write(k, v, k_cache, v_cache, slots)
 
 
@@ -84,10 +86,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     without tokens, or with no score above -inf, are 0.  A row is NaN where the table
     names a page outside the cache (nothing is read through it) or is too short for
     ``lens``.  Caches as for ``kv_write``; on a GPU their pages, heads and slots start
-    at multiples of 16 bytes.  An infinite value makes its column of the row infinite, and NaN where
-    its weight is 0 in fp32 or the sum holds both infinities; finite values below
-    2^120 / tokens leave the sums finite.  ``max_len`` (host) is a hint of the longest
-    sequence, for the split of the work alone."""
+    at multiples of 16 bytes.  An infinite value makes its column of the row infinite,
+    and NaN where its weight is 0 in fp32 or the sum holds both infinities; finite
+    values below 2^120 / tokens leave the sums finite.  ``max_len`` (host) is a hint of
+    the longest sequence, for the split of the work alone."""
     return _ops().paged_attention(q, k_cache, v_cache, table, lens, k, v, scale, max_len)
 
 

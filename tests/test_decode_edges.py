@@ -452,3 +452,12 @@ def test_attention_fp32_variants(device, kv_heads, group, dim, page, lens, appen
     _close(out, want, bound)
     if append:
         assert torch.equal(dk.cpu(), wk) and torch.equal(dv.cpu(), wv)
+
+
+@pytest.mark.parametrize("dtype,requests,beams,vocab,keep", [(BF, 2, 16, 20011, 64), (FP, 1, 40, 301, 64),
+                                                             (HF, 3, 9, 33333, 48), (BF, 1, 1, 50262, 64)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_select_many_places(device, dtype, requests, beams, vocab, keep):
+    """More candidates than the second kernel holds, most of which the waves' bound lets pass."""
+    x = (3 * torch.randn(requests, beams, vocab, generator=_g(keep + vocab))).to(dtype)
+    _selects(device, x, torch.randn(requests, beams, generator=_g(2)), keep)
