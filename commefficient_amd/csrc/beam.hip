@@ -46,6 +46,7 @@ namespace commeff {
 namespace {
 
 constexpr int kThreads = 256;
+static_assert(kBeamWaves == kThreads / 64, "a sum of every wave");
 constexpr int kPieces = 8;   // 16-byte pieces of a row that a thread holds
 constexpr int kList = 256;   // candidates of a wave that are ranked by counting
 constexpr int kJoinList = 1024;  // .. of the join
